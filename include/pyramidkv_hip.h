@@ -380,6 +380,127 @@ int pkv_ragged_attn_fwd_ws(const pkv_attn_args *args, void *workspace, int64_t w
 int pkv_ragged_attn_fwd_for(const pkv_attn_args *args, void *workspace, int64_t workspace_bytes,
                             pkv_stream_t stream);
 
+/* ---- rotary positions --------------------------------------------------- */
+
+enum pkv_dtype { PKV_DTYPE_BF16 = 0, PKV_DTYPE_FP16 = 1, PKV_DTYPE_FP32 = 2 };
+
+#define PKV_ROTARY_MAX_AXES 4
+
+/* Rotation of q [rows, num_heads_q, head_dim] and k [rows, num_heads_k,
+ * head_dim] (either may have no heads) into the contiguous q_out / k_out,
+ * which must not overlap the inputs.  pos holds num_axes positions a row
+ * (int64, or int32 with pos_is_int64 == 0); the first axis_pairs[0] pairs of a
+ * head turn by the first, the next axis_pairs[1] by the second, ...: pair j by
+ * pos * freqs[j] radians (freqs: one double a pair, on the device), times
+ * scale; by the opposite angle with inverse.  Pairs are neighbouring columns
+ * (interleaved) or columns j and j + pairs; columns from twice the pairs on are
+ * copied.  head_dim even, at most 256 pairs; strides in elements, the columns
+ * of a head dense. */
+typedef struct pkv_rotary_args {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const void *pos;
+  const double *freqs;
+  int64_t rows;
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride;
+  int32_t num_heads_q, num_heads_k, head_dim;
+  int32_t num_axes;
+  int32_t axis_pairs[PKV_ROTARY_MAX_AXES];
+  int32_t pos_is_int64, interleaved, inverse;
+  int32_t dtype; /* enum pkv_dtype */
+  float scale;
+} pkv_rotary_args;
+
+int pkv_rotary(const pkv_rotary_args *args, pkv_stream_t stream);
+
+/* ---- attention over chosen blocks of the cache --------------------------- */
+
+/* Keys and values as pkv_attn_args has them, for num_heads_kv KV heads, each
+ * serving num_heads_q / num_heads_kv query heads (head h of q belongs to KV head
+ * h / group): with kv_per_head the key sequence of (b, KV head h) is number
+ * s = b*num_heads_kv + h, otherwise s = b, and it begins at row
+ * cu_seqlens_k[s].  It has cu_seqlens_k[s + 1] - cu_seqlens_k[s] keys, or the
+ * first seqlens_k[s] of those rows where seqlens_k is given (a cache that
+ * grows in place).  Its blocks are block_k keys each (the last may be partial);
+ * block j is row cu_seqlens_k[s] / block_k + s + j of the block means, of
+ * total_k / block_k + num_seqs rows.  A query sequence's tiles are block_q
+ * tokens each; tile i of sequence b is row cu_seqlens_q[b] / block_q + b + i
+ * of the lists, of total_q / block_q + num_batches rows, each [num_heads_kv,
+ * topk] int32.  block_k: a multiple of 64 up to 1,024; block_q: 1 or more, with at
+ * most 256 rows (block_q * group) a tile; topk 1 to 1,024; head_dim 64 or 128;
+ * dtype bf16 or fp16.  causal (block_q 1 only): query i of a sequence of n sees
+ * its keys up to keys - n + i. */
+
+/* The mean of every block's keys, in fp32: means [rows, KV heads, head_dim]
+ * (one head a row with kv_per_head).  num_seqs key sequences.  last 0: rows
+ * without keys become zero.  last n > 0: only the blocks that hold one of a
+ * sequence's last n keys are written.  max_seqlen_k: a bound of a sequence's
+ * keys that sizes the launch (0: unknown). */
+typedef struct pkv_block_means_args {
+  const uint16_t *k;
+  float *means;
+  const int32_t *cu_seqlens_k, *seqlens_k;
+  int64_t total_k;
+  int64_t kv_tok_stride, kv_head_stride;
+  int32_t num_seqs, num_heads, head_dim, block_k;
+  int32_t last, max_seqlen_k;
+  int32_t dtype;
+} pkv_block_means_args;
+
+int pkv_block_means(const pkv_block_means_args *args, pkv_stream_t stream);
+
+/* The blocks that each tile attends to: the topk of its KV sequence's blocks by
+ * the product of the tile's summed query rows with the block's mean, the
+ * sums in 64 bits and the product rounded to fp32 (ties: the lower index; NaN
+ * counts as -inf), the first sink_blocks and last recent_blocks always among
+ * them; ascending, padded with -1.  Rows that are no tile's are -1.  Blocks past
+ * max_seqlen_k keys are not considered, tiles past max_seqlen_q have none.
+ * The workspace (pkv_block_select_workspace_size bytes, no initialisation)
+ * must not be shared by calls that may overlap. */
+typedef struct pkv_block_select_args {
+  const uint16_t *q;
+  const float *means;
+  int32_t *lists;
+  const int32_t *cu_seqlens_q, *cu_seqlens_k, *seqlens_k;
+  int64_t total_q, total_k;
+  int64_t q_tok_stride, q_head_stride;
+  int32_t num_batches, num_heads_q, num_heads_kv, head_dim, kv_per_head;
+  int32_t max_seqlen_q, max_seqlen_k;
+  int32_t block_q, block_k, topk, sink_blocks, recent_blocks, causal;
+  int32_t dtype;
+} pkv_block_select_args;
+
+int64_t pkv_block_select_workspace_size(const pkv_block_select_args *args);
+int pkv_block_select(const pkv_block_select_args *args, void *workspace, int64_t workspace_bytes, pkv_stream_t stream);
+
+/* Attention of each tile over the blocks of its list, o [total_q, num_heads_q,
+ * head_dim] and, if not NULL, the natural logarithm of each row's softmax sum,
+ * lse [num_heads_q, total_q].  Entries below 0, past the sequence's blocks or
+ * repeated are passed over, in any order.  A row without keys is 0 with lse
+ * -inf; one whose keys all score -inf is NaN.  Rows that no sequence owns, or
+ * past max_seqlen_q in theirs, are left as they were.  The workspace
+ * (pkv_block_attn_workspace_size bytes, possibly 0, no initialisation) must not
+ * be shared by calls that may overlap. */
+typedef struct pkv_block_attn_args {
+  const uint16_t *q, *k, *v;
+  uint16_t *o;
+  float *lse;
+  const int32_t *lists;
+  const int32_t *cu_seqlens_q, *cu_seqlens_k, *seqlens_k;
+  int64_t total_q, total_k;
+  int64_t q_tok_stride, q_head_stride;
+  int64_t kv_tok_stride, kv_head_stride;
+  int64_t o_tok_stride, o_head_stride;
+  int32_t num_batches, num_heads_q, num_heads_kv, head_dim, kv_per_head;
+  int32_t max_seqlen_q;
+  int32_t block_q, block_k, topk, causal;
+  float softmax_scale; /* above 0 */
+  int32_t dtype;
+} pkv_block_attn_args;
+
+int64_t pkv_block_attn_workspace_size(const pkv_block_attn_args *args);
+int pkv_block_attn(const pkv_block_attn_args *args, void *workspace, int64_t workspace_bytes, pkv_stream_t stream);
+
 /* ---- fused MegaCache.update -------------------------------------------- */
 
 /* Bytes of device workspace pkv_cache_update needs for F frames per block.

@@ -5,12 +5,13 @@
 // arguments like the reference, then calls the C ABI of
 // libpyramidkv_hip.so (include/pyramidkv_hip.h) with raw device pointers and
 // the current HIP stream.  Ops added by this build (ragged_attention,
-// rope_apply, cache_update, mega_merge_accum_weighted and the dit_* row
-// operations of the end-to-end rollout's model) are registered in
-// the same namespace.
+// rope_apply, rotary, cache_update, mega_merge_accum_weighted, the block_*
+// operators of attention over chosen blocks and the dit_* row operations of
+// the end-to-end rollout's model) are registered in the same namespace.
 
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/custom_class.h>
 #include <torch/library.h>
@@ -763,6 +764,298 @@ static Tensor rope_apply(Tensor k, Tensor pos, Tensor ft, Tensor fy, Tensor fx) 
   return out;
 }
 
+// ---- rotary positions and attention over chosen blocks
+static int32_t dtype_code(const Tensor &t, bool fp32, const char *who) {
+  if (t.scalar_type() == at::kBFloat16) return PKV_DTYPE_BF16;
+  if (t.scalar_type() == at::kHalf) return PKV_DTYPE_FP16;
+  TORCH_CHECK(fp32 && t.scalar_type() == at::kFloat, who, ": tensors must be bf16", fp32 ? ", fp16 or fp32" : " or fp16",
+              " (got ", t.scalar_type(), ")");
+  return PKV_DTYPE_FP32;
+}
+
+static int32_t to_i32(int64_t v, const char *who, const char *name) {
+  TORCH_CHECK(v >= -0x7fffffffLL - 1 && v <= 0x7fffffffLL, who, ": ", name, " (", v, ") exceeds 32 bits");
+  return static_cast<int32_t>(v);
+}
+
+// A [rows, heads, head_dim] (or, 2-D, [rows, head_dim]) operand on like's device
+// whose heads' columns are dense and whose rows the kernels can address.
+static void check_rows(const Tensor &t, const Tensor &like, const char *who, const char *name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), who, ": ", name, " must be on ", like.device(), " (got ",
+              t.device(), ")");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), who, ": ", name, " must be ", like.scalar_type(), " (got ",
+              t.scalar_type(), ")");
+  TORCH_CHECK(t.numel() == 0 || t.stride(-1) == 1, who, ": head_dim of ", name, " must be dense");
+}
+
+// rows that the kernels read in 16-byte accesses
+static void check_aligned(const Tensor &t, const char *who, const char *name) {
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, who, ": ", name, " must begin at 16 bytes");
+}
+
+static const int32_t *lens_or_null(const c10::optional<Tensor> &t, int64_t n, const Tensor &like, const char *who) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->device() == like.device(), who, ": seqlens_k must be on ", like.device());
+  check_i32(*t, "seqlens_k");
+  TORCH_CHECK(t->numel() == n, who, ": seqlens_k must have ", n, " entries (got ", t->numel(), ")");
+  return t->data_ptr<int32_t>();
+}
+
+static void check_cu(const Tensor &t, const Tensor &like, const char *who, const char *name) {
+  TORCH_CHECK(t.device() == like.device(), who, ": ", name, " must be on ", like.device(), " (got ", t.device(), ")");
+  check_i32(t, name);
+  TORCH_CHECK(t.dim() == 1 && t.numel() >= 1, who, ": ", name, " must have at least one entry");
+}
+
+static std::vector<Tensor> rotary(Tensor q, c10::optional<Tensor> k, Tensor pos, Tensor freqs, at::IntArrayRef axes,
+                                  bool interleaved, double scale, bool inverse) {
+  const char *who = "rotary";
+  const bool has_k = k.has_value() && k->defined();
+  TORCH_CHECK(q.is_cuda(), who, ": tensors must be on the GPU");
+  const int32_t dtype = dtype_code(q, true, who);
+  TORCH_CHECK(q.dim() == 3, who, ": q must be [rows, heads, head_dim]");
+  check_rows(q, q, who, "q");
+  if (has_k) {
+    check_rows(*k, q, who, "k");
+    TORCH_CHECK(k->dim() == 3 && k->size(0) == q.size(0) && k->size(2) == q.size(2), who,
+                ": k must be [rows, heads, head_dim] with q's rows and head_dim");
+  }
+  const int64_t n = q.size(0), A = static_cast<int64_t>(axes.size());
+  TORCH_CHECK(A >= 1 && A <= PKV_ROTARY_MAX_AXES, who, ": 1 to ", PKV_ROTARY_MAX_AXES, " axes (got ", A, ")");
+  int64_t pairs = 0;
+  for (int64_t p : axes) {
+    TORCH_CHECK(p >= 0, who, ": an axis cannot have ", p, " pairs");
+    pairs += p;
+  }
+  TORCH_CHECK(pairs >= 1 && 2 * pairs <= q.size(2), who, ": ", pairs, " pairs in heads of ", q.size(2));
+  TORCH_CHECK(freqs.device() == q.device() && freqs.scalar_type() == at::kDouble && freqs.is_contiguous() &&
+                  freqs.dim() == 1 && freqs.numel() == pairs,
+              who, ": freqs must be contiguous float64 [", pairs, "] on ", q.device());
+  TORCH_CHECK(pos.device() == q.device() && (pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) &&
+                  pos.is_contiguous(),
+              who, ": positions must be contiguous int64 or int32 on ", q.device());
+  TORCH_CHECK((pos.dim() == 2 && pos.size(0) == n && pos.size(1) == A) || (pos.dim() == 1 && A == 1 && pos.size(0) == n),
+              who, ": positions must be [", n, ", ", A, "] (got ", pos.sizes(), ")");
+  c10::DeviceGuard guard(q.device());
+  std::vector<Tensor> out = {at::empty(q.sizes(), q.options())};
+  if (has_k) out.push_back(at::empty(k->sizes(), k->options()));
+  pkv_rotary_args a{};
+  a.q = q.data_ptr();
+  a.q_out = out[0].data_ptr();
+  a.q_tok_stride = q.stride(0);
+  a.q_head_stride = q.stride(1);
+  a.num_heads_q = to_i32(q.numel() ? q.size(1) : 0, who, "heads");
+  if (has_k) {
+    a.k = k->data_ptr();
+    a.k_out = out[1].data_ptr();
+    a.k_tok_stride = k->stride(0);
+    a.k_head_stride = k->stride(1);
+    a.num_heads_k = to_i32(k->numel() ? k->size(1) : 0, who, "heads");
+  }
+  a.pos = pos.data_ptr();
+  a.pos_is_int64 = pos.scalar_type() == at::kLong ? 1 : 0;
+  a.freqs = freqs.data_ptr<double>();
+  a.rows = n;
+  a.head_dim = to_i32(q.size(2), who, "head_dim");
+  a.num_axes = static_cast<int32_t>(A);
+  for (int64_t i = 0; i < A; ++i) a.axis_pairs[i] = to_i32(axes[i], who, "pairs");
+  a.interleaved = interleaved ? 1 : 0;
+  a.inverse = inverse ? 1 : 0;
+  a.dtype = dtype;
+  a.scale = static_cast<float>(scale);
+  pkv_check(pkv_rotary(&a, stream_for(q)), who);
+  return out;
+}
+
+// k: [total_k, D] of one sequence per (batch, head), or [total_k, heads, D]
+static void run_block_means(const Tensor &means, const Tensor &k, const Tensor &cu, int64_t block_k, int64_t last,
+                            int64_t max_seqlen_k, const c10::optional<Tensor> &seqlens_k, const char *who) {
+  const int64_t S = cu.numel() - 1;
+  pkv_block_means_args a{};
+  a.k = reinterpret_cast<const uint16_t *>(k.data_ptr());
+  a.means = means.data_ptr<float>();
+  a.cu_seqlens_k = cu.data_ptr<int32_t>();
+  a.seqlens_k = lens_or_null(seqlens_k, S, k, who);
+  a.total_k = k.size(0);
+  a.kv_tok_stride = k.size(0) > 1 ? k.stride(0) : 0;
+  a.kv_head_stride = k.dim() == 3 && k.size(1) > 1 ? k.stride(1) : 0;
+  a.num_seqs = to_i32(S, who, "sequences");
+  a.num_heads = to_i32(k.dim() == 3 ? k.size(1) : 1, who, "heads");
+  a.head_dim = to_i32(k.size(-1), who, "head_dim");
+  a.block_k = to_i32(block_k, who, "block_k");
+  a.last = to_i32(last, who, "last");
+  a.max_seqlen_k = to_i32(max_seqlen_k, who, "max_seqlen_k");
+  a.dtype = dtype_code(k, false, who);
+  pkv_check(pkv_block_means(&a, stream_for(k)), who);
+}
+
+static void check_means_args(const Tensor &k, const Tensor &cu, int64_t block_k, const char *who) {
+  TORCH_CHECK(k.is_cuda(), who, ": tensors must be on the GPU");
+  dtype_code(k, false, who);
+  TORCH_CHECK(k.dim() == 2 || k.dim() == 3, who, ": k must be [total_k, D] or [total_k, heads, D]");
+  TORCH_CHECK(k.dim() == 2 || k.size(1) > 0, who, ": k must have heads");
+  check_rows(k, k, who, "k");
+  check_aligned(k, who, "k");
+  check_cu(cu, k, who, "cu_seqlens_k");
+  TORCH_CHECK(block_k > 0, who, ": block_k must be positive");
+}
+
+static std::vector<int64_t> means_shape(const Tensor &k, int64_t seqs, int64_t block_k) {
+  std::vector<int64_t> s = {k.size(0) / block_k + seqs};
+  if (k.dim() == 3) s.push_back(k.size(1));
+  s.push_back(k.size(-1));
+  return s;
+}
+
+static Tensor block_means(Tensor k, Tensor cu_seqlens_k, int64_t block_k, int64_t max_seqlen_k,
+                          c10::optional<Tensor> seqlens_k) {
+  const char *who = "block_means";
+  check_means_args(k, cu_seqlens_k, block_k, who);
+  c10::DeviceGuard guard(k.device());
+  Tensor means = at::empty(means_shape(k, cu_seqlens_k.numel() - 1, block_k), k.options().dtype(at::kFloat));
+  run_block_means(means, k, cu_seqlens_k, block_k, 0, max_seqlen_k, seqlens_k, who);
+  return means;
+}
+
+static void block_means_(Tensor means, Tensor k, Tensor cu_seqlens_k, int64_t block_k, int64_t last,
+                         int64_t max_seqlen_k, c10::optional<Tensor> seqlens_k) {
+  const char *who = "block_means_";
+  check_means_args(k, cu_seqlens_k, block_k, who);
+  const std::vector<int64_t> shape = means_shape(k, cu_seqlens_k.numel() - 1, block_k);
+  TORCH_CHECK(means.device() == k.device() && means.scalar_type() == at::kFloat && means.is_contiguous() &&
+                  means.sizes() == at::IntArrayRef(shape),
+              who, ": means must be contiguous float32 ", at::IntArrayRef(shape), " on ", k.device());
+  TORCH_CHECK(last >= 1, who, ": last must be at least 1");
+  c10::DeviceGuard guard(k.device());
+  run_block_means(means, k, cu_seqlens_k, block_k, last, max_seqlen_k, seqlens_k, who);
+}
+
+// KV heads that key sequences per head, or means / k of three dimensions, say
+static int64_t kv_heads_of(const Tensor &kv, int64_t cu_entries, int64_t B, const char *who) {
+  if (kv.dim() == 3) {
+    TORCH_CHECK(cu_entries == B + 1, who, ": cu_seqlens_k must have num_batches+1 entries");
+    return kv.size(1);
+  }
+  TORCH_CHECK(kv.dim() == 2, who, ": keys must be [rows, D] or [rows, heads, D]");
+  if (B == 0) return 1;
+  TORCH_CHECK(cu_entries > 1 && (cu_entries - 1) % B == 0, who,
+              ": per-head KV needs num_batches*heads+1 cu_seqlens_k entries");
+  return (cu_entries - 1) / B;
+}
+
+static Tensor block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int64_t max_seqlen_q,
+                           int64_t max_seqlen_k, int64_t topk, int64_t block_q, int64_t block_k, int64_t sink_blocks,
+                           int64_t recent_blocks, bool causal, c10::optional<Tensor> seqlens_k) {
+  const char *who = "block_select";
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, who, ": q must be a GPU tensor [total_q, heads, head_dim]");
+  check_rows(q, q, who, "q");
+  check_aligned(q, who, "q");
+  check_cu(cu_seqlens_q, q, who, "cu_seqlens_q");
+  check_cu(cu_seqlens_k, q, who, "cu_seqlens_k");
+  const int64_t B = cu_seqlens_q.numel() - 1, S = cu_seqlens_k.numel() - 1;
+  TORCH_CHECK(means.device() == q.device() && means.scalar_type() == at::kFloat && means.is_contiguous() &&
+                  (means.dim() == 2 || means.dim() == 3) && means.size(-1) == q.size(2),
+              who, ": means must be contiguous float32 [rows, (heads,) head_dim] on ", q.device());
+  check_aligned(means, who, "means");
+  const int64_t Hkv = kv_heads_of(means, S + 1, B, who);
+  TORCH_CHECK(block_q > 0 && block_k > 0 && topk > 0, who, ": block_q, block_k and topk must be positive");
+  TORCH_CHECK(Hkv > 0 && means.size(0) >= S, who, ": means has too few rows for ", S, " sequences");
+  pkv_block_select_args a{};
+  a.q = reinterpret_cast<const uint16_t *>(q.data_ptr());
+  a.means = means.data_ptr<float>();
+  a.cu_seqlens_q = cu_seqlens_q.data_ptr<int32_t>();
+  a.cu_seqlens_k = cu_seqlens_k.data_ptr<int32_t>();
+  a.seqlens_k = lens_or_null(seqlens_k, S, q, who);
+  a.total_q = q.size(0);
+  a.total_k = (means.size(0) - S) * block_k + block_k - 1;  // (the most keys whose means these can be)
+  a.q_tok_stride = q.size(0) > 1 ? q.stride(0) : 0;
+  a.q_head_stride = q.size(1) > 1 ? q.stride(1) : 0;
+  a.num_batches = to_i32(B, who, "batches");
+  a.num_heads_q = to_i32(q.size(1), who, "heads");
+  a.num_heads_kv = to_i32(Hkv, who, "KV heads");
+  a.head_dim = to_i32(q.size(2), who, "head_dim");
+  a.kv_per_head = means.dim() == 2 ? 1 : 0;
+  a.max_seqlen_q = to_i32(max_seqlen_q, who, "max_seqlen_q");
+  a.max_seqlen_k = to_i32(max_seqlen_k, who, "max_seqlen_k");
+  a.block_q = to_i32(block_q, who, "block_q");
+  a.block_k = to_i32(block_k, who, "block_k");
+  a.topk = to_i32(topk, who, "topk");
+  a.sink_blocks = to_i32(sink_blocks, who, "sink_blocks");
+  a.recent_blocks = to_i32(recent_blocks, who, "recent_blocks");
+  a.causal = causal ? 1 : 0;
+  a.dtype = dtype_code(q, false, who);
+  c10::DeviceGuard guard(q.device());
+  Tensor lists = at::empty({q.size(0) / block_q + B, Hkv, topk}, q.options().dtype(at::kInt));
+  a.lists = lists.data_ptr<int32_t>();
+  const int64_t need = pkv_block_select_workspace_size(&a);
+  Tensor ws = at::empty({need}, q.options().dtype(at::kByte));
+  pkv_check(pkv_block_select(&a, ws.data_ptr(), need, stream_for(q)), who);
+  return lists;
+}
+
+static std::vector<Tensor> block_sparse_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k,
+                                                  int64_t max_seqlen_q, Tensor lists, double softmax_scale,
+                                                  int64_t block_q, int64_t block_k, bool causal, bool return_lse,
+                                                  c10::optional<Tensor> seqlens_k) {
+  const char *who = "block_sparse_attention";
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, who, ": q must be a GPU tensor [total_q, heads, head_dim]");
+  check_rows(q, q, who, "q");
+  check_rows(k, q, who, "k");
+  check_rows(v, q, who, "v");
+  check_aligned(q, who, "q");
+  check_aligned(k, who, "k");
+  check_aligned(v, who, "v");
+  check_cu(cu_seqlens_q, q, who, "cu_seqlens_q");
+  check_cu(cu_seqlens_k, q, who, "cu_seqlens_k");
+  TORCH_CHECK(k.strides() == v.strides() && k.sizes() == v.sizes(), who, ": k and v must share a layout");
+  const int64_t B = cu_seqlens_q.numel() - 1, S = cu_seqlens_k.numel() - 1;
+  const int64_t Hkv = kv_heads_of(k, S + 1, B, who);
+  TORCH_CHECK(k.size(-1) == q.size(2), who, ": k and v must have q's head_dim");
+  TORCH_CHECK(block_q > 0, who, ": block_q must be positive");
+  TORCH_CHECK(lists.device() == q.device() && lists.scalar_type() == at::kInt && lists.is_contiguous() &&
+                  lists.dim() == 3 && lists.size(0) == q.size(0) / block_q + B && lists.size(1) == Hkv,
+              who, ": lists must be contiguous int32 [", q.size(0) / block_q + B, ", ", Hkv, ", topk] on ", q.device(),
+              " (got ", lists.sizes(), ")");
+  pkv_block_attn_args a{};
+  a.q = reinterpret_cast<const uint16_t *>(q.data_ptr());
+  a.k = reinterpret_cast<const uint16_t *>(k.data_ptr());
+  a.v = reinterpret_cast<const uint16_t *>(v.data_ptr());
+  a.lists = lists.data_ptr<int32_t>();
+  a.cu_seqlens_q = cu_seqlens_q.data_ptr<int32_t>();
+  a.cu_seqlens_k = cu_seqlens_k.data_ptr<int32_t>();
+  a.seqlens_k = lens_or_null(seqlens_k, S, q, who);
+  a.total_q = q.size(0);
+  a.total_k = k.size(0);
+  a.q_tok_stride = q.size(0) > 1 ? q.stride(0) : 0;
+  a.q_head_stride = q.size(1) > 1 ? q.stride(1) : 0;
+  a.kv_tok_stride = k.size(0) > 1 ? k.stride(0) : k.size(-1);
+  a.kv_head_stride = k.dim() == 3 && k.size(1) > 1 ? k.stride(1) : 0;
+  a.num_batches = to_i32(B, who, "batches");
+  a.num_heads_q = to_i32(q.size(1), who, "heads");
+  a.num_heads_kv = to_i32(Hkv, who, "KV heads");
+  a.head_dim = to_i32(q.size(2), who, "head_dim");
+  a.kv_per_head = k.dim() == 2 ? 1 : 0;
+  a.max_seqlen_q = to_i32(max_seqlen_q, who, "max_seqlen_q");
+  a.block_q = to_i32(block_q, who, "block_q");
+  a.block_k = to_i32(block_k, who, "block_k");
+  a.topk = to_i32(lists.size(2), who, "topk");
+  a.causal = causal ? 1 : 0;
+  a.softmax_scale = static_cast<float>(softmax_scale);
+  a.dtype = dtype_code(q, false, who);
+  c10::DeviceGuard guard(q.device());
+  std::vector<Tensor> out = {at::empty(q.sizes(), q.options())};
+  if (return_lse) out.push_back(at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat)));
+  a.o = reinterpret_cast<uint16_t *>(out[0].data_ptr());
+  a.o_tok_stride = out[0].stride(0);
+  a.o_head_stride = out[0].stride(1);
+  a.lse = return_lse ? out[1].data_ptr<float>() : nullptr;
+  const int64_t need = pkv_block_attn_workspace_size(&a);
+  Tensor ws;
+  if (need > 0) ws = at::empty({need}, q.options().dtype(at::kByte));
+  pkv_check(pkv_block_attn(&a, need > 0 ? ws.data_ptr() : nullptr, need, stream_for(q)), who);
+  return out;
+}
+
 // ---- DiT block row operations (the end-to-end rollout's model around the cache)
 static const float *f32_or_null(const c10::optional<Tensor> &t, int64_t n, const Tensor &like, const char *who) {
   if (!t.has_value() || !t->defined()) return nullptr;
@@ -1225,6 +1518,28 @@ static Tensor attn(Tensor q, Tensor, Tensor, Tensor, Tensor, int64_t, double, bo
   return at::empty_like(q);
 }
 static Tensor rope(Tensor k, Tensor, Tensor, Tensor, Tensor) { return at::empty_like(k); }
+static std::vector<Tensor> rotary(Tensor q, c10::optional<Tensor> k, Tensor, Tensor, at::IntArrayRef, bool, double,
+                                  bool) {
+  std::vector<Tensor> out = {at::empty(q.sizes(), q.options())};
+  if (k.has_value() && k->defined()) out.push_back(at::empty(k->sizes(), k->options()));
+  return out;
+}
+static Tensor block_means(Tensor k, Tensor cu, int64_t block_k, int64_t, c10::optional<Tensor>) {
+  return at::empty(adahead::means_shape(k, cu.numel() - 1, block_k), k.options().dtype(at::kFloat));
+}
+static void block_means_(Tensor, Tensor, Tensor, int64_t, int64_t, int64_t, c10::optional<Tensor>) {}
+static Tensor block_select(Tensor q, Tensor means, Tensor cu_q, Tensor cu_k, int64_t, int64_t, int64_t topk,
+                           int64_t block_q, int64_t, int64_t, int64_t, bool, c10::optional<Tensor>) {
+  const int64_t B = cu_q.numel() - 1;
+  return at::empty({q.size(0) / block_q + B, adahead::kv_heads_of(means, cu_k.numel(), B, "block_select"), topk},
+                   q.options().dtype(at::kInt));
+}
+static std::vector<Tensor> block_sparse_attention(Tensor q, Tensor, Tensor, Tensor, Tensor, int64_t, Tensor, double,
+                                                  int64_t, int64_t, bool, bool lse, c10::optional<Tensor>) {
+  std::vector<Tensor> out = {at::empty(q.sizes(), q.options())};
+  if (lse) out.push_back(at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat)));
+  return out;
+}
 static Tensor dit_ln(Tensor x, c10::optional<Tensor>, c10::optional<Tensor>, bool, double) {
   return at::empty(x.sizes(), x.options().dtype(at::kBFloat16));
 }
@@ -1357,6 +1672,17 @@ TORCH_LIBRARY(adahead, m) {
   m.def("ragged_attention_workspace_size() -> int");
   m.def("rope_apply(Tensor k, Tensor pos, Tensor freqs_ft_flat, Tensor freqs_fy_flat, Tensor freqs_fx_flat) "
         "-> Tensor");
+  m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor freqs, int[] axes, bool interleaved, float scale, "
+        "bool inverse) -> Tensor[]");
+  m.def("block_means(Tensor k, Tensor cu_seqlens_k, int block_k, int max_seqlen_k=0, Tensor? seqlens_k=None) -> Tensor");
+  m.def("block_means_(Tensor(a!) means, Tensor k, Tensor cu_seqlens_k, int block_k, int last, int max_seqlen_k=0, "
+        "Tensor? seqlens_k=None) -> ()");
+  m.def("block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, "
+        "int max_seqlen_k, int topk, int block_q, int block_k, int sink_blocks=0, int recent_blocks=0, "
+        "bool causal=False, Tensor? seqlens_k=None) -> Tensor");
+  m.def("block_sparse_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, "
+        "int max_seqlen_q, Tensor lists, float softmax_scale, int block_q, int block_k, bool causal=False, "
+        "bool return_lse=False, Tensor? seqlens_k=None) -> Tensor[]");
   m.def("dit_layer_norm(Tensor x, Tensor? mul, Tensor? add, bool mul_plus_one, float eps) -> Tensor");
   m.def("dit_rms_norm(Tensor x, Tensor? weight, float eps) -> Tensor");
   m.def("dit_residual_(Tensor(a!) x, Tensor y, Tensor? gate) -> ()");
@@ -1392,6 +1718,11 @@ TORCH_LIBRARY_IMPL(adahead, CUDA, m) {
   m.impl("mega_evict_merge", adahead::mega_evict_merge);
   m.impl("ragged_attention", adahead::ragged_attention);
   m.impl("rope_apply", adahead::rope_apply);
+  m.impl("rotary", adahead::rotary);
+  m.impl("block_means", adahead::block_means);
+  m.impl("block_means_", adahead::block_means_);
+  m.impl("block_select", adahead::block_select);
+  m.impl("block_sparse_attention", adahead::block_sparse_attention);
   m.impl("dit_layer_norm", adahead::dit_layer_norm);
   m.impl("dit_rms_norm", adahead::dit_rms_norm);
   m.impl("dit_residual_", adahead::dit_residual_);
@@ -1429,6 +1760,11 @@ TORCH_LIBRARY_IMPL(adahead, Meta, m) {
   m.impl("mega_plan_multi", adahead_meta::plan_multi);
   m.impl("ragged_attention", adahead_meta::attn);
   m.impl("rope_apply", adahead_meta::rope);
+  m.impl("rotary", adahead_meta::rotary);
+  m.impl("block_means", adahead_meta::block_means);
+  m.impl("block_means_", adahead_meta::block_means_);
+  m.impl("block_select", adahead_meta::block_select);
+  m.impl("block_sparse_attention", adahead_meta::block_sparse_attention);
   m.impl("dit_layer_norm", adahead_meta::dit_ln);
   m.impl("dit_rms_norm", adahead_meta::dit_rms);
   m.impl("dit_residual_", adahead_meta::dit_residual);

@@ -81,6 +81,39 @@ class UpdateArgs(ctypes.Structure):
                 ("workspace", _c_p), ("merge_heads", ctypes.c_uint64)]
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [("q", _c_p), ("k", _c_p), ("q_out", _c_p), ("k_out", _c_p), ("pos", _c_p), ("freqs", _c_p),
+                ("rows", _c_i64), ("q_tok_stride", _c_i64), ("q_head_stride", _c_i64), ("k_tok_stride", _c_i64),
+                ("k_head_stride", _c_i64), ("num_heads_q", _c_i32), ("num_heads_k", _c_i32), ("head_dim", _c_i32),
+                ("num_axes", _c_i32), ("axis_pairs", _c_i32 * 4), ("pos_is_int64", _c_i32), ("interleaved", _c_i32),
+                ("inverse", _c_i32), ("dtype", _c_i32), ("scale", _c_f)]
+
+
+class BlockMeansArgs(ctypes.Structure):
+    _fields_ = [("k", _c_p), ("means", _c_p), ("cu_seqlens_k", _c_p), ("seqlens_k", _c_p), ("total_k", _c_i64),
+                ("kv_tok_stride", _c_i64), ("kv_head_stride", _c_i64), ("num_seqs", _c_i32), ("num_heads", _c_i32),
+                ("head_dim", _c_i32), ("block_k", _c_i32), ("last", _c_i32), ("max_seqlen_k", _c_i32),
+                ("dtype", _c_i32)]
+
+
+class BlockSelectArgs(ctypes.Structure):
+    _fields_ = [("q", _c_p), ("means", _c_p), ("lists", _c_p), ("cu_seqlens_q", _c_p), ("cu_seqlens_k", _c_p),
+                ("seqlens_k", _c_p), ("total_q", _c_i64), ("total_k", _c_i64), ("q_tok_stride", _c_i64),
+                ("q_head_stride", _c_i64)] + [(n, _c_i32) for n in (
+                    "num_batches", "num_heads_q", "num_heads_kv", "head_dim", "kv_per_head", "max_seqlen_q",
+                    "max_seqlen_k", "block_q", "block_k", "topk", "sink_blocks", "recent_blocks", "causal", "dtype")]
+
+
+class BlockAttnArgs(ctypes.Structure):
+    _fields_ = [("q", _c_p), ("k", _c_p), ("v", _c_p), ("o", _c_p), ("lse", _c_p), ("lists", _c_p),
+                ("cu_seqlens_q", _c_p), ("cu_seqlens_k", _c_p), ("seqlens_k", _c_p), ("total_q", _c_i64),
+                ("total_k", _c_i64), ("q_tok_stride", _c_i64), ("q_head_stride", _c_i64), ("kv_tok_stride", _c_i64),
+                ("kv_head_stride", _c_i64), ("o_tok_stride", _c_i64), ("o_head_stride", _c_i64)] + [
+                    (n, _c_i32) for n in ("num_batches", "num_heads_q", "num_heads_kv", "head_dim", "kv_per_head",
+                                          "max_seqlen_q", "block_q", "block_k", "topk", "causal")] + [
+                    ("softmax_scale", _c_f), ("dtype", _c_i32)]
+
+
 _lib = None
 
 
@@ -116,6 +149,10 @@ def lib():
         L.pkv_ragged_attn_workspace_bound.argtypes = [ctypes.POINTER(AttnArgs), _c_i64]
         L.pkv_ragged_attn_fwd_ws.argtypes = [_c_p, _c_p, _c_i64, _c_p]
         L.pkv_ragged_attn_fwd_for.argtypes = [_c_p, _c_p, _c_i64, _c_p]
+        L.pkv_block_select_workspace_size.restype = _c_i64
+        L.pkv_block_select.argtypes = [_c_p, _c_p, _c_i64, _c_p]
+        L.pkv_block_attn_workspace_size.restype = _c_i64
+        L.pkv_block_attn.argtypes = [_c_p, _c_p, _c_i64, _c_p]
         _lib = L
     return _lib
 

@@ -32,6 +32,7 @@ import torch
 
 from . import _mega_state_ops, _mega_state_ref as ref, _ops
 from .base import HeadComposition
+from .block_sparse import BlockSparse, sparse_ragged_attention
 from .cyclic import CyclicStrategy
 from .lag import LagStrategy
 from .merge import MergeStrategy
@@ -211,8 +212,10 @@ class MegaCache:
                 int(ctx.sink_time_clamp_max), int(ctx.decoupled_sink_time_lag), *parts)
 
     def attend(self, q: torch.Tensor, current_start: int, *, freqs=None, softmax_scale=None, causal=False,
-               max_seqlen_k=None) -> torch.Tensor:
-        """Attention of q [1, L_q, H, D] (RoPE applied) over the cache."""
+               max_seqlen_k=None, sparse: BlockSparse | None = None) -> torch.Tensor:
+        """Attention of q [1, L_q, H, D] (RoPE applied) over the cache; with
+        ``sparse`` each tile of a chunk's queries over its best-scored blocks of
+        the packed keys alone (block_sparse.py)."""
         ctx = self.ctx
         FSEQ = ctx.frame_seqlen
         B, L_q, H, D = q.shape
@@ -224,6 +227,9 @@ class MegaCache:
             cu_q = ctx.cu_q[L_q] = torch.arange(0, L_q + 1, FSEQ, dtype=torch.int32, device=q.device)
         qb = q[0] if q.dtype == torch.bfloat16 else q[0].to(torch.bfloat16)
         max_keys = self._max_keys(int(current_start // FSEQ) + C)
+        if sparse is not None:
+            return self._attend_sparse(qb, cu_q, C, current_start, freqs, softmax_scale, causal,
+                                       sparse).view(1, L_q, H, D).to(q.dtype)
         if C <= int(ctx.mgr.max_attend_chunks()):
             scale = float(softmax_scale) if softmax_scale is not None else D ** -0.5
             out = ctx.mgr.attend_layer(*self._attend_args(current_start, C, freqs), qb, cu_q, scale, bool(causal),
@@ -234,6 +240,20 @@ class MegaCache:
                                         cu_k, FSEQ, softmax_scale, kv_per_head=True, causal=causal,
                                         workspace=self._split_workspace(q.device), max_seqlen_k=max_keys)
         return out.view(1, L_q, H, D).to(q.dtype)
+
+    def _attend_sparse(self, q, cu_q, C, current_start, freqs, softmax_scale, causal, sparse):
+        if causal:
+            raise RuntimeError("MegaCache.attend: the pyramid cache attends non-causally")
+        mgr, H, D = self.ctx.mgr, self.ctx.num_heads, self.ctx.head_dim
+        if C <= int(mgr.max_attend_chunks()):
+            cu_k = self.attend_kv(current_start, C, freqs)
+        else:
+            cu_k = self.pack(self.plan(current_start, C), freqs)
+        # the most keys that a (chunk, head) can pack, and the workspace rows that so many chunks can fill
+        max_keys = int(mgr.max_pack_tokens()) // (int(mgr.max_attend_chunks()) * H)
+        n = min(int(mgr.max_pack_tokens()), C * H * max_keys)
+        return sparse_ragged_attention(q, mgr.k_flat_out().view(-1, D)[:n], mgr.v_flat_out().view(-1, D)[:n], cu_q, cu_k,
+                                       self.ctx.frame_seqlen, max_keys, sparse, softmax_scale=softmax_scale)
 
     def _max_keys(self, frames: int) -> int:
         """The most keys that a head can hold once `frames` frames have come: a

@@ -10,8 +10,13 @@
   (torch.ops.adahead.rope_apply); replaces rope.py:18-68 and the Triton
   kernel of triton_rope.py.
 * ``map_sink_time`` / ``map_dynamic_pos_time``: rope.py:86-134.
+* ``rotary`` / ``rotary_frequencies``: rotation of q and k heads at any
+  position, without a table: both pair layouts, part of a head, one or several
+  position axes, frequencies scaled for long contexts, with its gradient.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -65,6 +70,84 @@ def apply_rope_to_flat_k(k_flat: torch.Tensor, pos_3d: torch.Tensor, freqs: torc
         out.copy_(res)
         return out
     return res
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
+                       trained_length: int = 0, fast_turns: float = 32.0, slow_turns: float = 1.0, device=None):
+    """(frequencies [rotary_dim / 2] float64, scale) for ``rotary``: pair j
+    turns by theta^(-2j / rotary_dim) radians a position.  scaling, for contexts
+    ``factor`` times as long as those trained on:
+
+    * "linear": every frequency divided by the factor;
+    * "base": theta raised so that the slowest pair is slowed by the factor and
+      the fastest not at all;
+    * "parts": pairs of more than ``fast_turns`` turns within ``trained_length``
+      positions as they are, those of fewer than ``slow_turns`` divided by the
+      factor, a linear blend by turns between them, and rotated q and k scaled
+      by 0.1 ln(factor) + 1 each."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_frequencies: rotary_dim ({rotary_dim}) must be even and at least 2")
+    if factor < 1.0:
+        raise ValueError(f"rotary_frequencies: factor ({factor}) must be at least 1")
+    j = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim
+    if scaling == "base":
+        if rotary_dim > 2:
+            theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+        return theta ** -j, 1.0
+    f = theta ** -j
+    if scaling is None:
+        return f, 1.0
+    if scaling == "linear":
+        return f / factor, 1.0
+    if scaling != "parts":
+        raise ValueError(f"rotary_frequencies: unknown scaling {scaling!r}")
+    if trained_length <= 0 or fast_turns <= slow_turns:
+        raise ValueError("rotary_frequencies: parts needs trained_length, and fast_turns above slow_turns")
+    turns = trained_length * f / (2 * math.pi)
+    keep = ((turns - slow_turns) / (fast_turns - slow_turns)).clamp(0, 1)
+    return f * keep + f / factor * (1 - keep), 0.1 * math.log(factor) + 1.0
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, freqs, axes, interleaved, scale, inverse):
+        ctx.save_for_backward(positions, freqs)
+        ctx.args = (axes, interleaved, scale, inverse)
+        out = _ops.ops().rotary(q, k, positions, freqs, axes, interleaved, scale, inverse)
+        return out[0] if k is None else tuple(out)
+
+    @staticmethod
+    def backward(ctx, gq, gk=None):
+        positions, freqs = ctx.saved_tensors
+        axes, interleaved, scale, inverse = ctx.args
+        dense = lambda g: g if g is None or g.stride(-1) == 1 else g.contiguous()
+        gq, gk = dense(gq), dense(gk)
+        if gq is None and gk is None:
+            return (None,) * 8
+        if gq is None or gk is None:  # one of them was not used, or there is no k
+            g = _Rotary.apply(gk if gq is None else gq, None, positions, freqs, axes, interleaved, scale, not inverse)
+            return (None, g) + (None,) * 6 if gq is None else (g,) + (None,) * 7
+        return _Rotary.apply(gq, gk, positions, freqs, axes, interleaved, scale, not inverse) + (None,) * 6
+
+
+def rotary(q: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, k: torch.Tensor | None = None, axes=None,
+           interleaved: bool = True, scale: float = 1.0, inverse: bool = False):
+    """Rotate the heads of q [rows, heads, D] (and of k, in the same launch) by
+    their rows' positions; bf16, fp16 or fp32, slices of a fused projection as
+    they lie.  Returns the rotated q, or (q, k).
+
+    positions [rows] or [rows, A] (int64 or int32): the first axes[0] pairs of a
+    head turn by the first column, the next axes[1] by the second, ... (default:
+    all by one).  freqs: float64, one a pair (rotary_frequencies); angles are
+    taken in 64 bits, so positions may be far.  Pair j is columns 2j and 2j + 1
+    (interleaved) or j and j + pairs; columns from twice the pairs on are
+    copied.  inverse turns back.  Differentiable in q and k."""
+    axes = (int(freqs.numel()),) if axes is None else tuple(int(a) for a in axes)
+    args = (positions, freqs, axes, bool(interleaved), float(scale), bool(inverse))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, *args)
+    out = _ops.ops().rotary(q, k, *args)
+    return out[0] if k is None else tuple(out)
 
 
 def map_sink_time(sync_t_raw: int, sink_time_mapping_mode: str, sink_time_clamp_min: int,
