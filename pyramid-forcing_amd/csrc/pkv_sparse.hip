@@ -144,6 +144,7 @@ struct SelectParams {
   int most, nb;    // blocks of the longest key sequence; a row of keys: the next multiple of 64
   int bq, bk, topk, sink, recent, causal;
   int tile0, tile_n;  // the tiles of every sequence that this launch takes
+  int chunks;         // workgroups that share a tile group's blocks
   double *sums;    // [B, tile_n, Hkv, D] or NULL: summed by the score kernel itself
   uint32_t *keys;  // [B, tile_n, Hkv, nb]
 };
@@ -170,47 +171,71 @@ __device__ inline int chosen_from(const SelectParams &p, const TileKeys &t) {
   return static_cast<int>(min(static_cast<int64_t>(min(t.blocks, p.most)), max(p.mean_rows - t.first, static_cast<int64_t>(0))));
 }
 
-// 8 columns from d on of the tile's rows, added up in fp64
+// 8 columns from d on of the tile's rows `from`, from + step, ..., added up in
+// fp64, kAhead rows read together (rows past the last repeat it and count 0)
 template <bool F16>
-__device__ inline void sum_rows(const SelectParams &p, int b, int h, int tile, int q_begin, int Lq, int d, int from,
-                                int step, double (&acc)[8]) {
-  const int rows = min(p.bq, Lq - tile * p.bq) * p.G;
+__device__ inline void sum_rows(const SelectParams &p, int h, int tile, const Span &q, int d, int from, int step,
+                                double (&acc)[8]) {
+  constexpr int kAhead = 4;
+  const int rows = min(p.bq, q.n - tile * p.bq) * p.G;
+  const uint16_t *base = p.q + (q.begin + static_cast<int64_t>(tile) * p.bq) * p.q_tok + h * p.G * p.q_head + d;
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.0;
-  for (int r = from; r < rows; r += step) {
-    const int t = r / p.G, g = r - t * p.G;
-    const uint4 v = *reinterpret_cast<const uint4 *>(p.q + (q_begin + static_cast<int64_t>(tile) * p.bq + t) * p.q_tok +
-                                                     (h * p.G + g) * p.q_head + d);
-    const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
+  for (int r0 = from; r0 < rows; r0 += kAhead * step) {
+    uint4 v[kAhead];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[2 * e] += static_cast<double>(elem_f32<F16>(static_cast<uint16_t>(wd[e] & 0xffff)));
-      acc[2 * e + 1] += static_cast<double>(elem_f32<F16>(static_cast<uint16_t>(wd[e] >> 16)));
+    for (int i = 0; i < kAhead; ++i) {
+      const int r = min(r0 + i * step, rows - 1), t = r / p.G;
+      v[i] = *reinterpret_cast<const uint4 *>(base + t * p.q_tok + (r - t * p.G) * p.q_head);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const uint32_t keep = r0 + i * step < rows ? 0xffffffffu : 0u;
+      const uint32_t wd[4] = {v[i].x & keep, v[i].y & keep, v[i].z & keep, v[i].w & keep};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[2 * e] += static_cast<double>(elem_f32<F16>(static_cast<uint16_t>(wd[e] & 0xffff)));
+        acc[2 * e + 1] += static_cast<double>(elem_f32<F16>(static_cast<uint16_t>(wd[e] >> 16)));
+      }
     }
   }
 }
 
-// the tile's summed query rows: one workgroup per (tile, KV head)
+// x + its value 16 (32) lanes away, in both
+__device__ inline double add_lane16(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const auto lo = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) +
+         __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+}
+__device__ inline double add_lane32(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const auto lo = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+  const auto hi = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) +
+         __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+}
+
+// the tile's summed query rows: grid (tiles, Hkv, B)
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) tile_sums_kernel(SelectParams p) {
   constexpr int LPR = D / 8, ROWS = 256 / LPR;
   __shared__ double part[ROWS][D + 1];
-  const int h = blockIdx.x % p.Hkv;
-  const int rest = blockIdx.x / p.Hkv;
-  const int b = rest / p.tile_n, tile = p.tile0 + rest % p.tile_n;
-  const Span rows_q = seq_span(p.cu_q, b, p.total_q);
-  const int q_begin = rows_q.begin, Lq = rows_q.n;
-  if (tile * p.bq >= Lq) return;
+  const int b = blockIdx.z, h = blockIdx.y, tile = p.tile0 + blockIdx.x;
+  const Span q = seq_span(p.cu_q, b, p.total_q);
+  if (tile * p.bq >= q.n) return;
   const int d = 8 * (threadIdx.x % LPR), sub = threadIdx.x / LPR;
   double acc[8];
-  sum_rows<F16>(p, b, h, tile, q_begin, Lq, d, sub, ROWS, acc);
+  sum_rows<F16>(p, h, tile, q, d, sub, ROWS, acc);
 #pragma unroll
   for (int e = 0; e < 8; ++e) part[sub][d + e] = acc[e];
   __syncthreads();
-  for (int c = threadIdx.x; c < D; c += 256) {
+  if (threadIdx.x < D) {
     double s = 0.0;
-    for (int r = 0; r < ROWS; ++r) s += part[r][c];
-    p.sums[static_cast<int64_t>(blockIdx.x) * D + c] = s;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) s += part[r][threadIdx.x];
+    p.sums[((static_cast<int64_t>(b) * p.tile_n + blockIdx.x) * p.Hkv + h) * D + threadIdx.x] = s;
   }
 }
 
@@ -220,49 +245,55 @@ __device__ inline uint32_t score_key(float f) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// grid: (block chunks, tile groups of 16, B * Hkv); 4 waves, each 16 blocks at
-// a time.  A operand: lane l holds tile l % 16, columns (l / 16) * D / 4 and
-// following; B operand: block l % 16, the same columns (the sum over the
-// columns may run in any order); result: lane l holds block l % 16 of tiles
-// l / 16 + 4 i.
+// grid: (tile groups of 16 * block chunks, Hkv, B); 4 waves, each 16 blocks at
+// a time.  A operand: lane l holds tile l % 16, columns 16 c + 4 (l / 16) + e (e
+// < 4, one matrix instruction each); B operand: block l % 16, the same columns,
+// so that the 4 lanes of a block read 64 bytes together (a lane's quarter of the
+// row in one piece had every read touch 64 cache lines, and again for each of
+// its 8 parts); result: lane l holds block l % 16 of tiles l / 16 + 4 i.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) block_scores_kernel(SelectParams p) {
   constexpr int C = D / 4;  // columns of a lane
-  const int b = blockIdx.z / p.Hkv, h = blockIdx.z % p.Hkv;
-  const Span rows_q = seq_span(p.cu_q, b, p.total_q);
-  const int q_begin = rows_q.begin, Lq = rows_q.n;
-  const int t0 = p.tile0 + blockIdx.y * 16;
-  const int last = min(min(t0 + 16, p.tile0 + p.tile_n), (Lq + p.bq - 1) / p.bq) - 1;  // the group's last tile
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int group = blockIdx.x / p.chunks, chunk = blockIdx.x - group * p.chunks;
+  const Span q = seq_span(p.cu_q, b, p.total_q);
+  const int t0 = p.tile0 + group * 16;
+  const int last = min(min(t0 + 16, p.tile0 + p.tile_n), (q.n + p.bq - 1) / p.bq) - 1;  // the group's last tile
+  const TileKeys tk = tile_keys(p, b, h, q.n, last);
   if (last < t0) return;
-  const TileKeys tk = tile_keys(p, b, h, Lq, last);
   const int blocks = chosen_from(p, tk);
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
-  int j = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
-  if (j >= blocks) return;
+  int j = (chunk * 4 + (threadIdx.x >> 6)) * 16;
+  if (chunk * 64 >= blocks) return;
 
   double qs[C];
   const int tile = min(t0 + i16, last);  // (lanes past the group's tiles repeat its last)
   if (p.sums) {
     const double *src =
-        p.sums + ((static_cast<int64_t>(b) * p.tile_n + tile - p.tile0) * p.Hkv + h) * D + g * C;
+        p.sums + ((static_cast<int64_t>(b) * p.tile_n + tile - p.tile0) * p.Hkv + h) * D + 4 * g;
 #pragma unroll
-    for (int c = 0; c < C; ++c) qs[c] = src[c];
+    for (int c = 0; c < C; ++c) qs[c] = src[16 * (c / 4) + c % 4];
   } else {
-#pragma unroll
-    for (int c = 0; c < C; c += 8) {
+    // thread i sums 8 columns of tile i / (D / 8)
+    __shared__ double sums[16][D + 2];
+    const int mine = threadIdx.x / (D / 8), d = 8 * (threadIdx.x % (D / 8));
+    if (mine < 16) {
       double acc[8];
-      sum_rows<F16>(p, b, h, tile, q_begin, Lq, g * C + c, 0, 1, acc);
+      sum_rows<F16>(p, h, min(t0 + mine, last), q, d, 0, 1, acc);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) qs[c + e] = acc[e];
+      for (int e = 0; e < 8; ++e) sums[mine][d + e] = acc[e];
     }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < C; ++c) qs[c] = sums[i16][16 * (c / 4) + 4 * g + c % 4];
   }
   const int width = p.per_head ? 1 : p.Hkv;
-  for (; j < blocks; j += gridDim.x * 64) {
+  for (; j < blocks; j += p.chunks * 64) {
     const int jj = min(j + i16, blocks - 1);
-    const float *m = p.means + ((tk.first + jj) * width + (p.per_head ? 0 : h)) * D + g * C;
+    const float *m = p.means + ((tk.first + jj) * width + (p.per_head ? 0 : h)) * D + 4 * g;
     float4 v[C / 4];
 #pragma unroll
-    for (int c = 0; c < C / 4; ++c) v[c] = *reinterpret_cast<const float4 *>(m + 4 * c);
+    for (int c = 0; c < C / 4; ++c) v[c] = *reinterpret_cast<const float4 *>(m + 16 * c);
     f64x4 s = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
     for (int c = 0; c < C / 4; ++c) {
@@ -281,46 +312,15 @@ __global__ void __launch_bounds__(256) block_scores_kernel(SelectParams p) {
   }
 }
 
-// The topk largest keys of a row of at most W * 64 * R, by W waves with R keys
-// a lane: wave w holds keys [w * 64 * R, ...), lane l of it keys l, l + 64,
-// ....  The topk-th largest is found bit by bit, counting with ballots; ties
-// at it go to the lowest indices.  One row per workgroup (W > 1), or 4
-// rows in 4 waves.
+// Writes the want = min(topk, n) largest of a row's keys, ascending by index and
+// padded with -1, to out.  W waves of R keys a lane take part: wave w holds keys
+// [w * 64 * R, ...), lane l of it keys l, l + 64, ...; 0 where there is none.
+// The want-th largest is found bit by bit, counting with ballots; ties at it go
+// to the lowest indices.  counts: 2 * W ints of LDS (W > 1, where the whole
+// workgroup calls it).
 template <int W, int R>
-__global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(SelectParams p) {
-  __shared__ int counts[2][W > 1 ? W : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = W > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  if (row >= static_cast<int64_t>(p.B) * p.tile_n * p.Hkv) return;
-  const int h = static_cast<int>(row % p.Hkv);
-  const int rest = static_cast<int>(row / p.Hkv);
-  const int b = rest / p.tile_n, tile = p.tile0 + rest % p.tile_n;
-  const Span rows_q = seq_span(p.cu_q, b, p.total_q);
-  const int q_begin = rows_q.begin, Lq = rows_q.n;
-  const int64_t first_row = q_begin / p.bq + b;
-  const int have = min((Lq + p.bq - 1) / p.bq, p.tiles);
-  if (tile == 0) {  // the rows behind the sequence's tiles
-    const int64_t end = b + 1 < p.B ? seq_span(p.cu_q, b + 1, p.total_q).begin / p.bq + b + 1 : p.tile_rows;
-    for (int64_t r = first_row + max(have, 0); r < end; ++r)
-      for (int e = W > 1 ? static_cast<int>(threadIdx.x) : lane; e < p.topk; e += W > 1 ? 64 * W : 64)
-        p.lists[(r * p.Hkv + h) * p.topk + e] = -1;
-  }
-  if (tile >= have) return;
-  const TileKeys tk = tile_keys(p, b, h, Lq, tile);
-  const int n = chosen_from(p, tk);
-  const uint32_t *src = p.keys + row * p.nb;
-  const int base = W > 1 ? wave * 64 * R : 0;
-  uint32_t key[R];  // 0: no such block
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int j = base + r * 64 + lane;
-    key[r] = j < n ? src[j] : 0u;
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int j = base + r * 64 + lane;
-    if (j < n && (j < p.sink || j >= n - p.recent)) key[r] = 0xffffffffu;
-  }
+__device__ inline void choose(const uint32_t (&key)[R], int n, int topk, int32_t *out, int *counts) {
+  const int lane = threadIdx.x & 63, wave = W > 1 ? threadIdx.x >> 6 : 0;
   int which = 0;
   // over the row: how many keys are at least x
   auto count = [&](uint32_t x) {
@@ -328,19 +328,19 @@ __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(Sele
 #pragma unroll
     for (int r = 0; r < R; ++r) c += __popcll(__builtin_amdgcn_ballot_w64(key[r] >= x));
     if constexpr (W > 1) {
-      if (lane == 0) counts[which][wave] = c;
+      if (lane == 0) counts[which * W + wave] = c;
       __syncthreads();
       c = 0;
 #pragma unroll
-      for (int w = 0; w < W; ++w) c += counts[which][w];
+      for (int w = 0; w < W; ++w) c += counts[which * W + w];
       which ^= 1;
     }
     return c;
   };
-  const int want = min(p.topk, n);
-  uint32_t at = 1;  // the want-th largest key
+  const int want = min(topk, n);
+  uint32_t at = 1;        // the want-th largest key
   int ties = W * 64 * R;  // how many of the keys equal to it are chosen
-  if (n > p.topk) {
+  if (n > topk) {
     at = 0;
     int reached = 0;
     for (int bit = 31; bit >= 0; --bit) {
@@ -354,7 +354,6 @@ __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(Sele
     }
     if (reached > want) ties = want - (at == 0xffffffffu ? 0 : count(at + 1));
   }
-  int32_t *out = p.lists + ((first_row + tile) * p.Hkv + h) * p.topk;
   int pos = 0, tied = 0;
   if constexpr (W > 1) {  // those of the waves before
     int above = 0, equal = 0;
@@ -365,13 +364,13 @@ __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(Sele
     }
     __syncthreads();
     if (lane == 0) {
-      counts[0][wave] = above;
-      counts[1][wave] = equal;
+      counts[wave] = above;
+      counts[W + wave] = equal;
     }
     __syncthreads();
     for (int w = 0; w < wave; ++w) {
-      pos += counts[0][w];
-      tied += counts[1][w];
+      pos += counts[w];
+      tied += counts[W + w];
     }
     pos += min(tied, ties);
   }
@@ -381,11 +380,155 @@ __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(Sele
     const uint64_t eq = __builtin_amdgcn_ballot_w64(key[r] == at);
     const bool take = key[r] > at || (key[r] == at && tied + __popcll(eq & below) < ties);
     const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
-    if (take) out[pos + __popcll(taken & below)] = base + r * 64 + lane;
+    if (take) out[pos + __popcll(taken & below)] = (wave * R + r) * 64 + lane;
     pos += __popcll(taken);
     tied += __popcll(eq);
   }
-  for (int e = want + (W > 1 ? static_cast<int>(threadIdx.x) : lane); e < p.topk; e += W > 1 ? 64 * W : 64) out[e] = -1;
+  for (int e = want + wave * 64 + lane; e < topk; e += 64 * W) out[e] = -1;
+}
+
+// The lists' rows behind sequence b's `have` tiles, for KV head h
+__device__ inline void clear_rows(const SelectParams &p, int b, int h, int64_t from, int thread, int threads) {
+  const int64_t end = b + 1 < p.B ? seq_span(p.cu_q, b + 1, p.total_q).begin / p.bq + b + 1 : p.tile_rows;
+  for (int64_t r = from; r < end; ++r)
+    for (int e = thread; e < p.topk; e += threads) p.lists[(r * p.Hkv + h) * p.topk + e] = -1;
+}
+
+// A row (tile, KV head) of the lists from block_scores_kernel's keys: one per
+// workgroup of W waves, or, W 1, one per wave and 4 per workgroup.  Grid: (tiles,
+// Hkv, B).
+template <int W, int R>
+__global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(SelectParams p) {
+  __shared__ int counts[2 * W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.z, h = blockIdx.y, nth = W > 1 ? blockIdx.x : blockIdx.x * 4 + wave, tile = p.tile0 + nth;
+  const Span q = seq_span(p.cu_q, b, p.total_q);
+  const TileKeys tk = tile_keys(p, b, h, q.n, tile);
+  const int64_t first_row = q.begin / p.bq + b;
+  const int have = min((q.n + p.bq - 1) / p.bq, p.tiles);
+  if (tile == 0)
+    clear_rows(p, b, h, first_row + have, W > 1 ? static_cast<int>(threadIdx.x) : lane, W > 1 ? 64 * W : 64);
+  if (tile >= have || nth >= p.tile_n) return;
+  const int n = chosen_from(p, tk);
+  const int64_t row = (static_cast<int64_t>(b) * p.tile_n + nth) * p.Hkv + h;
+  const uint32_t *src = p.keys + row * p.nb;
+  const int base = W > 1 ? wave * 64 * R : 0;
+  uint32_t key[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = base + r * 64 + lane;
+    key[r] = j < n ? src[j] : 0u;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = base + r * 64 + lane;
+    if (j < n && (j < p.sink || j >= n - p.recent)) key[r] = 0xffffffffu;
+  }
+  choose<W, R>(key, n, p.topk, p.lists + ((first_row + tile) * p.Hkv + h) * p.topk, counts);
+}
+
+// Scores and choice in one launch, where a row's blocks are few: W waves a row
+// (W 1: 4 rows a workgroup, each wave by itself), grid (tiles, Hkv, B).  The row's summed queries and
+// its keys lie in LDS; 4 lanes take a block's mean, 16 blocks a wave at a time,
+// in vector fp64.  A row of the lists costs nb * 4 D bytes of means, which the
+// rows of a sequence do not share as block_scores_kernel's 16 do.
+template <int D, bool F16, int W, int R>
+__global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_select_kernel(SelectParams p) {
+  constexpr int ROWS = W > 1 ? 1 : 4, NB = W * 64 * R;  // rows of a workgroup, keys of a row
+  constexpr int LPR = D / 8, SUB = 64 / LPR, C = D / 4;
+  __shared__ double sums[ROWS][W][D];
+  __shared__ uint32_t keys[ROWS][NB];
+  __shared__ int counts[2 * W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int slot = W > 1 ? 0 : wave, part = W > 1 ? wave : 0;
+  const int b = blockIdx.z, h = blockIdx.y, tile = W > 1 ? blockIdx.x : blockIdx.x * 4 + wave;
+  const Span q = seq_span(p.cu_q, b, p.total_q);
+  const TileKeys tk = tile_keys(p, b, h, q.n, tile);
+  const int64_t first_row = q.begin / p.bq + b;
+  const int have = min((q.n + p.bq - 1) / p.bq, p.tiles);
+  if (tile == 0)
+    clear_rows(p, b, h, first_row + have, W > 1 ? static_cast<int>(threadIdx.x) : lane, W > 1 ? 64 * W : 64);
+  if (tile >= have) return;
+  const int n = chosen_from(p, tk);
+  const int i16 = lane & 15, g = lane >> 4;
+  const int width = p.per_head ? 1 : p.Hkv;
+  const float *means = p.means + (tk.first * width + (p.per_head ? 0 : h)) * D + 4 * g;
+  auto fetch = [&](int j, float4 (&v)[C / 4]) {  // (blocks past the last repeat it)
+    const float *m = means + static_cast<int64_t>(min(j + i16, n - 1)) * width * D;
+#pragma unroll
+    for (int c = 0; c < C / 4; ++c) v[c] = *reinterpret_cast<const float4 *>(m + 16 * c);
+  };
+  constexpr int kAhead = 2;  // reads of 16 blocks in flight
+  float4 v[kAhead][C / 4];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)  // on their way while the queries are summed
+    if ((part + i * W) * 16 < n) fetch((part + i * W) * 16, v[i]);
+
+  const int sub = part * SUB + lane / LPR;
+  double acc[8];
+  sum_rows<F16>(p, h, tile, q, 8 * (lane % LPR), sub, W * SUB, acc);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (LPR == 8) acc[e] += __shfl_xor(acc[e], 8);
+    acc[e] = add_lane32(add_lane16(acc[e]));
+  }
+  if (lane < LPR)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[slot][part][8 * lane + e] = acc[e];
+  if constexpr (W > 1) {
+    __syncthreads();
+    if (threadIdx.x < D) {
+      double x = sums[0][0][threadIdx.x];
+#pragma unroll
+      for (int w = 1; w < W; ++w) x += sums[0][w][threadIdx.x];
+      sums[0][0][threadIdx.x] = x;
+    }
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  double qs[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) qs[c] = sums[slot][0][16 * (c / 4) + 4 * g + c % 4];
+  for (int j0 = part * 16; j0 < n; j0 += kAhead * 16 * W)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + i * 16 * W;
+      if (j >= n) break;
+      double s0 = 0.0, s1 = 0.0;
+#pragma unroll
+      for (int c = 0; c < C / 4; ++c) {
+        s0 = fma(qs[4 * c], static_cast<double>(v[i][c].x), s0);
+        s1 = fma(qs[4 * c + 1], static_cast<double>(v[i][c].y), s1);
+        s0 = fma(qs[4 * c + 2], static_cast<double>(v[i][c].z), s0);
+        s1 = fma(qs[4 * c + 3], static_cast<double>(v[i][c].w), s1);
+      }
+      if (j + kAhead * 16 * W < n) fetch(j + kAhead * 16 * W, v[i]);
+      const double s = add_lane32(add_lane16(s0 + s1));
+      const int at = j + i16;
+      if (g == 0 && at < n)
+        keys[slot][at] = at < p.sink || at >= n - p.recent ? 0xffffffffu : score_key(static_cast<float>(s));
+    }
+  if constexpr (W > 1) __syncthreads();
+  else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  int32_t *out = p.lists + ((first_row + tile) * p.Hkv + h) * p.topk;
+  // one wave where it holds the keys: no barriers in the search
+  if (W == 1 || n <= 512) {
+    if (W > 1 && wave > 0) return;
+    constexpr int R1 = W == 1 ? R : 8;
+    uint32_t key[R1];
+#pragma unroll
+    for (int r = 0; r < R1; ++r) key[r] = r * 64 + lane < n ? keys[slot][r * 64 + lane] : 0u;
+    choose<1, R1>(key, n, p.topk, out, counts);
+  } else {
+    uint32_t key[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int at = (wave * R + r) * 64 + lane;
+      key[r] = at < n ? keys[slot][at] : 0u;
+    }
+    choose<W, R>(key, n, p.topk, out, counts);
+  }
 }
 
 // ---- attention over the listed blocks -----------------------------------------
@@ -397,7 +540,8 @@ struct BlockAttnParams {
   int total_q, total_k;
   int64_t q_tok, q_head, kv_tok, kv_head, o_tok, o_head;
   int B, Hq, Hkv, G, per_head;
-  int tiles, items;  // tiles of the longest sequence; B * Hkv * tiles
+  int tiles, items;  // tiles (groups of tiles) of the longest sequence; B * Hkv * tiles
+  int group;         // tiles that a workgroup takes together
   int bq, bk, topk, causal;
   float scale_log2;
   int splits;        // workgroups of an item
@@ -540,8 +684,8 @@ constexpr float kSlack = 8.0f;
 
 // One wave's step over NK * 32 keys in LDS (K and V rows from kt / vt): S^T =
 // K Q^T, the probabilities against the row's moving reference, O^T += V^T P^T.
-// The first `keys` keys count.
-template <int D, int NK, bool F16>
+// The first `keys` keys count (LANES: of each lane's row its own).
+template <int D, int NK, bool F16, bool LANES = false>
 __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (&qf)[D / 16], int keys, float c,
                                    RowState<D> &st) {
   constexpr int ROW = 2 * D;
@@ -558,7 +702,7 @@ __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (
       s[kb] = mfma16<F16>(a, qf[x], s[kb]);
     }
   }
-  if (keys < 32 * NK) {
+  if (LANES ? __builtin_amdgcn_ballot_w64(keys < 32 * NK) != 0 : keys < 32 * NK) {
     asm volatile("");  // (kept a branch: whole tiles skip the compares)
 #pragma unroll
     for (int kb = 0; kb < NK; ++kb)
@@ -612,8 +756,8 @@ __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (
 }
 
 struct AttnTile {
-  int b, h, q_begin, Lq, tok0, rows, nsub;
-  TileKeys tk;
+  int b, h, q_begin, Lq, tok0, rows;
+  TileKeys tk;  // of the last tile
 };
 
 // item -> its tile; false where the sequence has no such tile
@@ -624,10 +768,11 @@ __device__ inline bool attn_tile(const BlockAttnParams &p, int item, AttnTile &t
   const Span q = seq_span(p.cu_q, t.b, p.total_q);
   t.q_begin = q.begin;
   t.Lq = q.n;
-  t.tok0 = tile * p.bq;
+  t.tok0 = tile * p.group * p.bq;
   if (t.tok0 >= t.Lq) return false;
-  t.rows = min(p.bq, t.Lq - t.tok0) * p.G;
-  t.tk = tile_keys(p, t.b, t.h, t.Lq, tile);
+  const int tokens = min(p.group * p.bq, t.Lq - t.tok0);
+  t.rows = tokens * p.G;
+  t.tk = tile_keys(p, t.b, t.h, t.Lq, (t.tok0 + tokens - 1) / p.bq);
   return true;
 }
 
@@ -674,23 +819,36 @@ __device__ inline void store_rows(const BlockAttnParams &p, const AttnTile &t, i
     p.lse[static_cast<int64_t>(head) * p.total_q + row] = l > 0.0f || l != l ? (st.m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
 }
 
-// Tiles of up to 32 W rows: W waves of 32 rows, the keys in steps of 64 through
-// two LDS buffers that all waves share.
+// Tiles of up to 32 W rows: W waves of 32 rows, the listed keys in steps of 32
+// through rings of four K and four V tiles in LDS that all waves share, one
+// barrier a step.  Step t computes S(t + 1) = K(t + 1) Q^T beside the
+// exponentials of P(t), independent of each other, then O += V(t)^T P(t); the
+// row maxima of S(t + 1) are taken last, so that the one branch of a step, the
+// rescale of O, lies at its end.  K(t + 4) and V(t + 3) are copied during step t into
+// the slots that step t - 1 was the last to read.
+//
+// What bounds it: a 32-row wave reads 16 KB of LDS fragments for 16 matrix
+// instructions of 32 cycles, which at 128 bytes a cycle for four SIMDs is the
+// same time; two workgroups a compute unit keep both busy.
+template <int N>
+using ic = std::integral_constant<int, N>;
+
 template <int D, int W, bool F16>
 __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnParams p) {
-  constexpr int ROW = 2 * D, TILE = kSub * ROW;  // bytes
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];  // K0 V0 K1 V1
-  __shared__ int list[kMaxTopk];
+  constexpr int ROW = 2 * D, TILE = 32 * ROW;  // bytes
+  __shared__ __attribute__((aligned(1024))) char smem[8 * TILE];  // four K tiles, four V tiles
+  __shared__ int list[kMaxTopk + 1];
   __shared__ int scratch[2];
   const int item = xcd_order(blockIdx.x, p.items);
   AttnTile t;
   if (!attn_tile(p, item, t)) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, lq = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = p.bk / kSub;
-  const int n = __builtin_amdgcn_readfirstlane(load_list<64 * W>(tile_list(p, t), p.topk, t.tk.blocks, list, scratch)) * per;
-
-  const int r = 32 * wave + (lane & 31);
+  const int blocks = __builtin_amdgcn_readfirstlane(
+      load_list<64 * W>(tile_list(p, t), p.topk, t.tk.blocks, list, scratch));
+  const int n = blocks * (p.bk / 32);  // steps
+  const int r = 32 * wave + lq;
+  const float c = p.scale_log2;
   uint4 qf[D / 16];
   load_query<D>(p, t, r, qf);
   wait_copies<0>();  // (no load of the compiler's own is then pending among the copies)
@@ -701,6 +859,193 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
     for (int i = 0; i < 16; ++i) st.o[db][i] = 0.0f;
   st.m = -INFINITY;
   st.l = 0.0f;
+  if (n == 0) {
+    store_rows<D, F16>(p, t, r, st, 0.0f, false);
+    return;
+  }
+
+  // ---- copies: a tile's K and V rows are 2 * CP copies of RPC rows each,
+  // PER of them a wave's, all of K or all of V
+  constexpr int RPC = 64 / (D / 8), CP = 32 / RPC, PER = 2 * CP / W;
+  static_assert(PER >= 1 && CP % PER == 0, "copies");
+  const int64_t head_off = p.per_head ? 0 : t.h * p.kv_head;
+  const bool of_v = wave * PER >= CP;
+  const uint16_t *src = (of_v ? p.v : p.k) + t.tk.begin * p.kv_tok + head_off;
+  const int row_bytes = static_cast<int>(p.kv_tok) * 2;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem)) + (of_v ? 4 * TILE : 0);
+  int voff[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int row = ((wave * PER + i) % CP) * RPC + lane / (D / 8), pos = lane % (D / 8);
+    voff[i] = row * row_bytes + 16 * (of_v ? v_chunk<D>(row, pos) : k_chunk<D>(row, pos));
+  }
+  // a step's first key, its block's end and its place in the list
+  struct Cursor {
+    int key, end, entry, next;  // next: the following block, read a block ahead
+  };
+  auto begin = [&]() {
+    const int key = __builtin_amdgcn_readfirstlane(list[0]) * p.bk;
+    return Cursor{key, key + p.bk, 0, list[1]};
+  };
+  auto advance = [&](Cursor &x) {
+    x.key += 32;
+    if (x.key == x.end) {  // (past the last block the list may hold anything: keys_of has none there)
+      ++x.entry;
+      x.key = __builtin_amdgcn_readfirstlane(x.next) * p.bk;
+      x.end = x.key + p.bk;
+      x.next = list[min(x.entry + 1, kMaxTopk)];
+    }
+  };
+  auto keys_of = [&](const Cursor &x) { return x.entry < blocks ? max(0, t.tk.limit - x.key) : 0; };
+  Cursor copied = begin(), masked = begin();
+  auto copy = [&](auto slot) {
+    const int left = min(32, keys_of(copied));
+    const int64_t off = left > 0 ? copied.key * p.kv_tok : 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      copy_rows(src + off, static_cast<int64_t>(left) * row_bytes,
+                lds0 + (decltype(slot)::value & 3) * TILE + ((wave * PER + i) % CP) * RPC * ROW, voff[i]);
+    advance(copied);
+  };
+
+  // ---- fragment addresses
+  int kaddr[D / 16], vaddr[D / 32];
+#pragma unroll
+  for (int x = 0; x < D / 16; ++x) kaddr[x] = lq * ROW + 16 * k_chunk<D>(lq, 2 * x + hf);
+  const int vr = 4 * hf + ((lane & 15) >> 2), vc = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) vaddr[db] = vr * ROW + 16 * v_chunk<D>(vr, 4 * db + vc / 8) + 2 * (vc % 8);
+  auto scores = [&](auto slot, f32x16 &s) {
+    uint4 kf[D / 16];
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x)
+      kf[x] = *reinterpret_cast<const uint4 *>(smem + (decltype(slot)::value & 3) * TILE + kaddr[x]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) s = mfma16<F16>(kf[x], qf[x], s);
+  };
+  // the keys past `keys` out, and the reference raised where a score is far above it
+  auto settle = [&](f32x16 &s, int keys) {
+    if (keys < 32) {
+      asm volatile("");  // (kept a branch: whole tiles skip the compares)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + 4 * hf + i % 4 >= keys) s[i] = -INFINITY;
+    }
+    float x = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) x = fmaxf(x, s[i]);
+    x = both_max(x) * c;
+    const bool raise = x > st.m + kSlack || (st.m == -INFINITY && x > -INFINITY);
+    if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+      const float f = raise ? __builtin_amdgcn_exp2f(st.m - x) : 1.0f;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[db][i] *= f;
+      st.l *= f;
+      st.m = raise ? x : st.m;
+    }
+  };
+  f32x16 sa, sb;
+  auto step = [&](auto tt) {
+    constexpr int T = decltype(tt)::value;
+    f32x16 &cur = T & 1 ? sb : sa;
+    f32x16 &nxt = T & 1 ? sa : sb;
+    scores(ic<T + 1>(), nxt);
+    const float ref = st.m == -INFINITY ? 0.0f : st.m;
+    typename Elem8<F16>::x8 pb[2];
+    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(cur[i], c, -ref));
+      (i & 1 ? l1 : l0) += e;
+      pb[i / 8][i % 8] = static_cast<typename Elem8<F16>::type>(e);
+    }
+    st.l += l0 + l1;
+    const char *vt = smem + (4 + T) * TILE;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) {
+        const char *p0 = vt + vaddr[db] + 16 * ks * ROW;
+        const i16x4 a8[2] = {lds_read_tr(p0), lds_read_tr(p0 + 8 * ROW)};  // (rows 8 apart lie alike)
+        st.o[db] = mfma16<F16>(__builtin_bit_cast(uint4, a8), __builtin_bit_cast(uint4, pb[ks]), st.o[db]);
+      }
+    settle(nxt, keys_of(masked));
+    advance(masked);
+  };
+  // two steps, T and T + 1, between barriers: what they read has arrived, and
+  // the slots that the two before read are free
+  auto turn = [&](auto tt) {
+    constexpr int T = decltype(tt)::value;
+    wait_copies<0>();
+    wait_reads();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (of_v) {
+      copy(ic<T + 2>());
+      copy(ic<T + 3>());
+    } else {
+      copy(ic<T + 3>());
+      copy(ic<T>());
+    }
+    step(ic<T>());
+    step(ic<T + 1>());
+  };
+  // K(0 .. 2) and V(0 .. 1)
+  copy(ic<0>());
+  copy(ic<1>());
+  if (!of_v) copy(ic<2>());
+  wait_copies<0>();
+  __syncthreads();
+  scores(ic<0>(), sa);
+  settle(sa, keys_of(masked));
+  advance(masked);
+  // whole turns of the rings: steps past the last copy zeros and mask every key
+  for (int s = 0; s < n; s += 4) {
+    turn(ic<0>());
+    turn(ic<2>());
+  }
+  wait_copies<0>();  // no copy may land in LDS after the workgroup ends
+  store_rows<D, F16>(p, t, r, st, both_sum(st.l), true);
+}
+
+// Several consecutive small tiles at once (a prompt in which every token has a
+// list of its own): a workgroup walks the union of their lists in steps of 64
+// keys through two buffers; a step counts for the rows whose tile lists its
+// block, and a wave none of whose rows do only copies.  Neighbouring tokens
+// share most of their blocks, so that the keys are copied for all of them at
+// once, and a wave of 32 rows, which a single small tile would not fill, does
+// no more matrix work than the tiles one by one.  A row gets 0 * V from
+// blocks that only its neighbours list: where that is not 0 (V holds an
+// infinity or NaN) the results say so, and the workgroup takes its tiles one by
+// one instead.
+constexpr int kWindow = 1024;    // blocks whose lists are joined at a time
+constexpr int kMaxGroup = 32;    // tiles: a bit each
+constexpr int kGroupItems = 256; // workgroups that a launch in groups has at least
+
+template <int D, int W, bool F16>
+__global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnParams p) {
+  constexpr int ROW = 2 * D, TILE = kSub * ROW;  // bytes
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];  // K0 V0 K1 V1
+  __shared__ int list[kWindow];
+  __shared__ uint32_t members[kWindow];  // of the window's blocks, the tiles that list them
+  __shared__ int scratch[W > 2 ? W : 2];
+  static_assert(kWindow % (64 * W) == 0, "window");
+  const int item = xcd_order(blockIdx.x, p.items);
+  AttnTile t;
+  if (!attn_tile(p, item, t)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per = p.bk / kSub;
+
+  const int r = 32 * wave + (lane & 31);
+  uint4 qf[D / 16];
+  load_query<D>(p, t, r, qf);
+  wait_copies<0>();  // (no load of the compiler's own is then pending among the copies)
+  RowState<D> st;
 
   const int64_t head_off = p.per_head ? 0 : t.h * p.kv_head;
   const uint16_t *kp = p.k + t.tk.begin * p.kv_tok + head_off;
@@ -710,13 +1055,11 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
   const int crow = lane / (D / 8), cpos = lane % (D / 8);
   const int row_bytes = static_cast<int>(p.kv_tok) * 2;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem));
-  auto first_key = [&](int s) {
-    const int blk = __builtin_amdgcn_readfirstlane(list[s / per]);
-    return blk * p.bk + (s % per) * kSub;
-  };
-  auto issue = [&](int s, int buf) {
+  auto block_of = [&](int s) { return __builtin_amdgcn_readfirstlane(list[s / per]); };
+  auto first_key = [&](int s) { return block_of(s) * p.bk + (s % per) * kSub; };
+  auto issue = [&](int s, int buf, int limit) {
     const int key = first_key(s);
-    const int64_t left = max(0, min(kSub, t.tk.limit - key));
+    const int64_t left = max(0, min(kSub, limit - key));
     const int64_t off = left > 0 ? key * p.kv_tok : 0;
     const uint32_t dst = lds0 + buf * 2 * TILE;
 #pragma unroll
@@ -727,17 +1070,108 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
       copy_rows(vp + off, left * row_bytes, at + TILE, row * row_bytes + 16 * v_chunk<D>(row, cpos));
     }
   };
-  if (n > 0) issue(0, 0);
-  for (int s = 0; s < n; ++s) {
-    wait_copies<0>();
-    wait_reads();
-    __builtin_amdgcn_s_barrier();  // step s has arrived, and no wave reads the other buffer any more
-    asm volatile("" ::: "memory");
-    if (s + 1 < n) issue(s + 1, (s + 1) & 1);
-    const char *kt = smem + (s & 1) * 2 * TILE;
-    attend_step<D, 2, F16>(kt, kt + TILE, qf, max(0, t.tk.limit - first_key(s)), p.scale_log2, st);
+  auto reset = [&]() {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[db][i] = 0.0f;
+    st.m = -INFINITY;
+    st.l = 0.0f;
+  };
+  // the steps of list[0 .. n / per), keys up to `limit`; step(s, tile in LDS)
+  auto walk = [&](int n, int limit, auto &&step) {
+    if (n > 0) issue(0, 0, limit);
+    for (int s = 0; s < n; ++s) {
+      wait_copies<0>();
+      wait_reads();
+      __builtin_amdgcn_s_barrier();  // step s has arrived, and no wave reads the other buffer any more
+      asm volatile("" ::: "memory");
+      if (s + 1 < n) issue(s + 1, (s + 1) & 1, limit);
+      step(s, smem + (s & 1) * 2 * TILE);
+    }
+  };
+  reset();
+
+  const int32_t *src = tile_list(p, t);
+  const int64_t row = static_cast<int64_t>(p.Hkv) * p.topk;
+  const int last = (t.rows / p.G - 1) / p.bq;  // the group's last tile, whose limit t.tk has
+  // keys that a tile may see (causal tiles are one token each)
+  auto limit_of = [&](int tile) { return p.causal ? max(0, t.tk.limit - (last - tile)) : t.tk.limit; };
+  const int my_tile = min(r, t.rows - 1) / p.G / p.bq;
+  const int my_limit = limit_of(my_tile);
+  uint32_t wave_tiles = 0;  // those that this wave has rows of
+  if (32 * wave < t.rows) {
+    const int lo = 32 * wave / p.G / p.bq, hi = min(32 * wave + 31, t.rows - 1) / p.G / p.bq;
+    wave_tiles = (0xffffffffu >> (31 - (hi - lo))) << lo;
   }
-  store_rows<D, F16>(p, t, r, st, both_sum(st.l), n > 0);
+  bool seen = false;  // whether this lane's row had a key
+  // walks the union of the lists, or tile `only`'s
+  auto pass = [&](int only) {
+    const int limit = only < 0 ? t.tk.limit : limit_of(only);
+    const uint32_t take = only < 0 ? 0xffffffffu : 1u << only;
+    for (int w0 = 0; w0 < t.tk.blocks; w0 += kWindow) {
+      __syncthreads();
+      for (int e = threadIdx.x; e < kWindow; e += 64 * W) members[e] = 0;
+      __syncthreads();
+      for (int e = threadIdx.x; e < (last + 1) * p.topk; e += 64 * W) {
+        const int tile = e / p.topk;
+        const int x = src[tile * row + (e - tile * p.topk)];
+        if (x >= w0 && x < w0 + kWindow && x < (limit_of(tile) + p.bk - 1) / p.bk)
+          atomicOr(&members[x - w0], (1u << tile) & take);
+      }
+      __syncthreads();
+      // the blocks that any tile lists, in order: each thread a run of them
+      constexpr int RUN = kWindow / (64 * W);
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) mine += members[threadIdx.x * RUN + i] != 0;
+      const int upto = wave_incl_sum(mine);
+      if (lane == 63) scratch[wave] = upto;
+      __syncthreads();
+      int at = upto - mine, n = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        at += w < wave ? scratch[w] : 0;
+        n += scratch[w];
+      }
+#pragma unroll
+      for (int i = 0; i < RUN; ++i)
+        if (members[threadIdx.x * RUN + i] != 0) list[at++] = w0 + threadIdx.x * RUN + i;
+      __syncthreads();
+      n = __builtin_amdgcn_readfirstlane(n);
+      walk(n * per, limit, [&](int s, const char *kt) {
+        const int blk = block_of(s);
+        const uint32_t who = __builtin_amdgcn_readfirstlane(members[blk - w0]);
+        if ((who & wave_tiles) == 0) return;
+        const int keys = (who >> my_tile) & 1 ? max(0, my_limit - first_key(s)) : 0;
+        seen = seen || keys > 0;
+        attend_step<D, 2, F16, true>(kt, kt + TILE, qf, keys, p.scale_log2, st);
+      });
+    }
+  };
+  pass(-1);
+  float check = st.l;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) check = fmaf(st.o[db][i], 0.0f, check);
+  const bool odd = __builtin_amdgcn_ballot_w64(r < t.rows && !(check - check == 0.0f)) != 0;
+  __syncthreads();
+  if (threadIdx.x == 0) scratch[0] = 0;
+  __syncthreads();
+  if (odd && lane == 0) scratch[0] = 1;
+  __syncthreads();
+  const bool again = __builtin_amdgcn_readfirstlane(scratch[0]) != 0;
+  if (!again) {
+    store_rows<D, F16>(p, t, r, st, both_sum(st.l), seen);
+    return;
+  }
+  for (int tile = 0; tile <= last; ++tile) {
+    reset();
+    seen = false;
+    pass(tile);
+    store_rows<D, F16>(p, t, my_tile == tile ? r : t.rows, st, both_sum(st.l), seen);
+  }
 }
 
 // Tiles of up to 32 rows (single tokens of grouped heads): 4 waves that each
@@ -989,7 +1423,20 @@ constexpr int kMaxSelectBlocks = 32768;
 
 struct SelectPlan {
   int64_t nb, tiles, tile_n, sums_bytes, bytes;
+  bool fused;
 };
+
+// Scores and choice in one launch where that reads few means more than once,
+// measured against three launches, microseconds each (head_dim 128):
+// * up to 128 blocks (a wave a row), up to kFusedBytes of means in all: 1,024
+//   rows of 64 blocks 7.6 against 11.3, 4,094 of 64 12.0 against 13.0, but
+//   32,768 of 64 97 against 33;
+// * more, where no other tile of the sequence reads the same means (single
+//   tokens) and the rows fill the chip: 128 rows of 512 blocks 14.4 against
+//   18.1, 512 of 2,048 106 against 124, but 8 of 2,048 37 against 19, and
+//   468 rows of 13 tiles a sequence and 320 blocks 21.7 against 16.8.
+constexpr int64_t kFusedBytes = 140ll << 20;
+constexpr int64_t kFusedMost = 4096, kFusedRows = 64;
 
 static int check_select(const pkv_block_select_args *a) {
   if (!a) return fail(PKV_ERR_INVALID, "block_select: NULL argument");
@@ -1003,8 +1450,8 @@ static int check_select(const pkv_block_select_args *a) {
                 a->topk);
   if ((static_cast<int64_t>(a->max_seqlen_k) + a->block_k - 1) / a->block_k > kMaxSelectBlocks)
     return fail(PKV_ERR_UNSUPPORTED, "block_select: more than %d blocks", kMaxSelectBlocks);
-  if (static_cast<int64_t>(a->num_batches) * a->num_heads_kv > 65535)
-    return fail(PKV_ERR_UNSUPPORTED, "block_select: more than 65535 KV heads of all batches");
+  if (a->num_batches > 65535 || a->num_heads_kv > 65535)
+    return fail(PKV_ERR_UNSUPPORTED, "block_select: more than 65535 batches or KV heads");
   if (a->total_q > 0x7fffffff) return fail(PKV_ERR_UNSUPPORTED, "block_select: too many query rows");
   return PKV_OK;
 }
@@ -1016,6 +1463,10 @@ static SelectPlan select_plan(const pkv_block_select_args *a) {
   if (s.nb == 0) s.nb = 64;
   if (s.tiles == 0) s.tiles = 1;  // (the lists' rows are written all the same)
   const int64_t heads = static_cast<int64_t>(a->num_batches) * a->num_heads_kv;
+  const int64_t rows = heads * s.tiles;
+  s.fused = s.nb <= 128 ? rows * s.nb * a->head_dim * 4 <= kFusedBytes
+                        : s.tiles == 1 && rows >= kFusedRows && s.nb <= kFusedMost;
+  if (s.fused) return s;
   const bool sums = a->block_q * (a->num_heads_q / a->num_heads_kv) > kSumRowsInline;
   const int64_t per_tile = heads * (s.nb * 4 + (sums ? a->head_dim * 8 : 0));
   s.tile_n = kSelectWorkspace / (per_tile > 0 ? per_tile : 1) / 16 * 16;
@@ -1029,13 +1480,25 @@ static SelectPlan select_plan(const pkv_block_select_args *a) {
 template <int D, bool F16>
 static int launch_select(const SelectParams &p0, const SelectPlan &s, hipStream_t st) {
   const int64_t heads = static_cast<int64_t>(p0.B) * p0.Hkv;
+  if (s.fused) {
+    SelectParams p = p0;
+    p.tile0 = 0;
+    p.tile_n = static_cast<int>(s.tiles);
+    if (s.nb <= 128) {
+      auto *k = s.nb <= 64 ? block_select_kernel<D, F16, 1, 1> : block_select_kernel<D, F16, 1, 2>;
+      hipLaunchKernelGGL(k, dim3((p.tile_n + 3) / 4, p.Hkv, p.B), dim3(256), 0, st, p);
+    } else {
+      auto *k = s.nb <= 512 ? block_select_kernel<D, F16, 8, 1> : block_select_kernel<D, F16, 8, 8>;
+      hipLaunchKernelGGL(k, dim3(p.tile_n, p.Hkv, p.B), dim3(512), 0, st, p);
+    }
+    return check_launch("block_select_kernel");
+  }
   for (int64_t tile0 = 0; tile0 < s.tiles; tile0 += s.tile_n) {
     SelectParams p = p0;
     p.tile0 = static_cast<int>(tile0);
     p.tile_n = static_cast<int>(s.tiles - tile0 < s.tile_n ? s.tiles - tile0 : s.tile_n);
-    const int64_t rows = heads * p.tile_n;
     if (p.sums) {
-      hipLaunchKernelGGL((tile_sums_kernel<D, F16>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((tile_sums_kernel<D, F16>), dim3(p.tile_n, p.Hkv, p.B), dim3(256), 0, st, p);
       if (const int rc = check_launch("tile_sums_kernel")) return rc;
     }
     const int64_t groups = (p.tile_n + 15) / 16;
@@ -1043,17 +1506,20 @@ static int launch_select(const SelectParams &p0, const SelectPlan &s, hipStream_
     int64_t chunks = (s.nb + 63) / 64;
     const int64_t most = (2048 + groups * heads - 1) / (groups * heads);
     if (chunks > most) chunks = most;
-    hipLaunchKernelGGL((block_scores_kernel<D, F16>),
-                       dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(groups), static_cast<unsigned>(heads)),
-                       dim3(256), 0, st, p);
+    p.chunks = static_cast<int>(chunks);
+    hipLaunchKernelGGL((block_scores_kernel<D, F16>), dim3(static_cast<unsigned>(groups * chunks), p.Hkv, p.B), dim3(256),
+                       0, st, p);
     if (const int rc = check_launch("block_scores_kernel")) return rc;
-    // the fewest waves that hold a row's keys in registers
-    if (s.nb <= 64 * 32) {
-      auto *k = s.nb <= 64 * 2 ? block_choose_kernel<1, 2> : s.nb <= 64 * 8 ? block_choose_kernel<1, 8> : block_choose_kernel<1, 32>;
-      hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, st, p);
+    // one wave up to 8 keys a lane (no barriers in the search), then the fewest
+    // that hold them
+    if (s.nb <= 64 * 8) {
+      auto *k = s.nb <= 64 * 2 ? block_choose_kernel<1, 2> : block_choose_kernel<1, 8>;
+      hipLaunchKernelGGL(k, dim3((p.tile_n + 3) / 4, p.Hkv, p.B), dim3(256), 0, st, p);
+    } else if (s.nb <= 256 * 8) {
+      hipLaunchKernelGGL((block_choose_kernel<4, 8>), dim3(p.tile_n, p.Hkv, p.B), dim3(256), 0, st, p);
     } else {
       auto *k = s.nb <= 1024 * 8 ? block_choose_kernel<16, 8> : block_choose_kernel<16, 32>;
-      hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(rows)), dim3(1024), 0, st, p);
+      hipLaunchKernelGGL(k, dim3(p.tile_n, p.Hkv, p.B), dim3(1024), 0, st, p);
     }
     if (const int rc = check_launch("block_choose_kernel")) return rc;
   }
@@ -1076,12 +1542,10 @@ extern "C" int pkv_block_select(const pkv_block_select_args *a, void *workspace,
   if ((a->q_tok_stride | a->q_head_stride) & 7)
     return fail(PKV_ERR_INVALID, "block_select: strides must keep 16-byte rows aligned");
   const SelectPlan s = select_plan(a);
-  if (!workspace || workspace_bytes < s.bytes)
+  if (s.bytes > 0 && (!workspace || workspace_bytes < s.bytes))
     return fail(PKV_ERR_CAPACITY, "block_select: workspace of %lld bytes, %lld needed",
                 static_cast<long long>(workspace_bytes), static_cast<long long>(s.bytes));
   const int64_t heads = static_cast<int64_t>(a->num_batches) * a->num_heads_kv;
-  if (heads * s.tile_n > 0x7fffffff || (s.tile_n + 15) / 16 > 65535)
-    return fail(PKV_ERR_UNSUPPORTED, "block_select: grid too large");
   SelectParams p{};
   p.q = a->q; p.means = a->means; p.lists = a->lists;
   p.cu_q = a->cu_seqlens_q; p.cu_k = a->cu_seqlens_k; p.used = a->seqlens_k;
@@ -1121,49 +1585,69 @@ static int check_attn(const pkv_block_attn_args *a) {
   return PKV_OK;
 }
 
-static int64_t attn_items(const pkv_block_attn_args *a) {
-  return static_cast<int64_t>(a->num_batches) * a->num_heads_kv *
-         ((static_cast<int64_t>(a->max_seqlen_q) + a->block_q - 1) / a->block_q);
-}
+// How a launch is cut: tiles that a workgroup takes together, workgroups that
+// share a tile.
+struct AttnPlan {
+  int64_t tiles, items;  // groups of a sequence, of all
+  int group, splits;
+};
 
-// Workgroups of a small tile: as many as give the chip one each, but at least
-// four 32-key steps a wave.
-static int attn_splits(const pkv_block_attn_args *a) {
-  if (a->block_q * (a->num_heads_q / a->num_heads_kv) > 32) return 1;
-  const int64_t items = attn_items(a);
-  if (items == 0) return 1;
-  int64_t s = 256 / items;
-  const int64_t most = static_cast<int64_t>(a->topk) * (a->block_k / 32) / (4 * kSmallWaves);
-  if (s > most) s = most;
-  return static_cast<int>(s < 1 ? 1 : s);
+static AttnPlan attn_plan(const pkv_block_attn_args *a) {
+  AttnPlan s{};
+  const int rows = a->block_q * (a->num_heads_q / a->num_heads_kv);
+  const int64_t heads = static_cast<int64_t>(a->num_batches) * a->num_heads_kv;
+  const int64_t tiles = (static_cast<int64_t>(a->max_seqlen_q) + a->block_q - 1) / a->block_q;
+  s.group = s.splits = 1;
+  if (rows <= 32) {
+    // as many tiles as make 128 rows, fewer where that leaves compute units
+    // without a workgroup
+    int64_t g = 128 / rows < kMaxGroup ? 128 / rows : kMaxGroup;
+    if (g > tiles) g = tiles;
+    while (g > 1 && heads * ((tiles + g - 1) / g) < kGroupItems) g /= 2;
+    if (g > 1) s.group = static_cast<int>(g);
+  }
+  s.tiles = (tiles + s.group - 1) / s.group;
+  s.items = heads * s.tiles;
+  if (rows <= 32 && s.group == 1 && s.items > 0) {
+    // as many workgroups as give the chip one each, but at least four 32-key
+    // steps a wave
+    int64_t n = 256 / s.items;
+    const int64_t most = static_cast<int64_t>(a->topk) * (a->block_k / 32) / (4 * kSmallWaves);
+    if (n > most) n = most;
+    if (n > 1) s.splits = static_cast<int>(n);
+  }
+  return s;
 }
 
 template <int D, bool F16>
 static int launch_block_attn(const BlockAttnParams &p, hipStream_t st) {
   const int rows = p.bq * p.G;
-  if (rows <= 32) {
-    hipLaunchKernelGGL((block_attn_small_kernel<D, F16>), dim3(p.items * p.splits), dim3(64 * kSmallWaves), 0, st, p);
-    if (const int rc = check_launch("block_attn_small_kernel")) return rc;
-    if (p.splits == 1) return PKV_OK;
-    const int64_t waves = static_cast<int64_t>(p.items) * rows;
-    hipLaunchKernelGGL((block_attn_join_kernel<D, F16>), dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, st, p);
-    return check_launch("block_attn_join_kernel");
+  if (p.group > 1) {
+    const bool two = p.group * rows <= 64;
+    hipLaunchKernelGGL((two ? block_attn_group_kernel<D, 2, F16> : block_attn_group_kernel<D, 4, F16>), dim3(p.items),
+                       dim3(two ? 128 : 256), 0, st, p);
+    return check_launch("block_attn_group_kernel");
   }
-  if (rows <= 64)
-    hipLaunchKernelGGL((block_attn_tile_kernel<D, 2, F16>), dim3(p.items), dim3(128), 0, st, p);
-  else if (rows <= 128)
-    hipLaunchKernelGGL((block_attn_tile_kernel<D, 4, F16>), dim3(p.items), dim3(256), 0, st, p);
-  else
-    hipLaunchKernelGGL((block_attn_tile_kernel<D, 8, F16>), dim3(p.items), dim3(512), 0, st, p);
-  return check_launch("block_attn_tile_kernel");
+  if (rows > 32) {
+    const int w = rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+    auto *k = w == 2 ? block_attn_tile_kernel<D, 2, F16> : w == 4 ? block_attn_tile_kernel<D, 4, F16> : block_attn_tile_kernel<D, 8, F16>;
+    hipLaunchKernelGGL(k, dim3(p.items), dim3(64 * w), 0, st, p);
+    return check_launch("block_attn_tile_kernel");
+  }
+  hipLaunchKernelGGL((block_attn_small_kernel<D, F16>), dim3(p.items * p.splits), dim3(64 * kSmallWaves), 0, st, p);
+  if (const int rc = check_launch("block_attn_small_kernel")) return rc;
+  if (p.splits == 1) return PKV_OK;
+  const int64_t waves = static_cast<int64_t>(p.items) * rows;
+  hipLaunchKernelGGL((block_attn_join_kernel<D, F16>), dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, st, p);
+  return check_launch("block_attn_join_kernel");
 }
 
 }  // namespace pkv
 
 extern "C" int64_t pkv_block_attn_workspace_size(const pkv_block_attn_args *a) {
   if (!a || check_attn(a)) return 0;
-  const int s = attn_splits(a);
-  return s > 1 ? attn_items(a) * s * 32 * (a->head_dim + 4) * 4 : 0;
+  const AttnPlan s = attn_plan(a);
+  return s.splits > 1 ? s.items * s.splits * 32 * (a->head_dim + 4) * 4 : 0;
 }
 
 extern "C" int pkv_block_attn(const pkv_block_attn_args *a, void *workspace, int64_t workspace_bytes,
@@ -1193,12 +1677,14 @@ extern "C" int pkv_block_attn(const pkv_block_attn_args *a, void *workspace, int
   p.B = a->num_batches; p.Hq = a->num_heads_q; p.Hkv = a->num_heads_kv;
   p.G = a->num_heads_q / a->num_heads_kv;
   p.per_head = a->kv_per_head ? 1 : 0;
-  p.tiles = static_cast<int>((static_cast<int64_t>(a->max_seqlen_q) + a->block_q - 1) / a->block_q);
-  p.items = static_cast<int>(attn_items(a));
+  const AttnPlan s = attn_plan(a);
+  p.tiles = static_cast<int>(s.tiles);
+  p.items = static_cast<int>(s.items);
+  p.group = s.group;
   p.bq = a->block_q; p.bk = a->block_k; p.topk = a->topk;
   p.causal = a->causal ? 1 : 0;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-  p.splits = attn_splits(a);
+  p.splits = s.splits;
   p.part = static_cast<float *>(workspace);
   hipStream_t st = as_stream(stream);
   const bool f16 = a->dtype == PKV_DTYPE_FP16;

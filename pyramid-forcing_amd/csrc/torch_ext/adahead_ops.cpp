@@ -988,8 +988,9 @@ static Tensor block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor c
   Tensor lists = at::empty({q.size(0) / block_q + B, Hkv, topk}, q.options().dtype(at::kInt));
   a.lists = lists.data_ptr<int32_t>();
   const int64_t need = pkv_block_select_workspace_size(&a);
-  Tensor ws = at::empty({need}, q.options().dtype(at::kByte));
-  pkv_check(pkv_block_select(&a, ws.data_ptr(), need, stream_for(q)), who);
+  Tensor ws;
+  if (need > 0) ws = at::empty({need}, q.options().dtype(at::kByte));
+  pkv_check(pkv_block_select(&a, need > 0 ? ws.data_ptr() : nullptr, need, stream_for(q)), who);
   return lists;
 }
 

@@ -82,9 +82,9 @@ def test_selection_refusals(fault):
 
 
 def test_selection_needs_its_workspace():
-    a = _select()
+    a = _select(max_seqlen_k=64 * 20000)  # (few blocks need none: scores and choice in one launch)
     need = A.lib().pkv_block_select_workspace_size(ctypes.byref(a))
-    assert need >= 64 * 4
+    assert need >= 20000 * 4 and A.lib().pkv_block_select_workspace_size(ctypes.byref(_select())) == 0
     _refused(A.lib().pkv_block_select(ctypes.byref(a), FAKE, need - 1, None))
     _refused(A.lib().pkv_block_select(ctypes.byref(a), None, need, None))
     assert A.lib().pkv_block_select_workspace_size(ctypes.byref(_select(head_dim=96))) == 0

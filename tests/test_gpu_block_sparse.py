@@ -323,6 +323,10 @@ ATTEND = [  # q lens, k lens, hkv, G, per_head, topk, bq, bk, causal
     ([257, 255], [1000, 3000], 1, 1, True, 7, 256, 64, False),
     ([100], [2000], 1, 3, False, 12, 85, 128, False),
     ([100], [2000], 1, 48, False, 3, 5, 64, False),
+    # many small tiles: several of them to a workgroup
+    ([700], [700], 2, 8, False, 6, 1, 64, True), ([310, 250], [900, 100], 2, 16, False, 5, 1, 64, True),
+    ([2047], [1500], 1, 16, False, 3, 1, 128, True), ([1000], [640], 3, 1, True, 4, 4, 64, False),
+    ([1030], [70000], 1, 8, False, 8, 2, 64, False), ([5, 900], [0, 300], 1, 7, False, 2, 3, 64, False),
 ]
 
 
@@ -345,6 +349,28 @@ def test_attend(case, D, dtype):
         again = bs.block_sparse_attention(q, k, v, cu(q_lens), cu(k_lens), max(q_lens), lists, block_q=bq, block_k=bk,
                                           causal=causal)
         assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("poison", [float("nan"), INF])
+def test_attend_neighbours_blocks(poison):
+    """Tiles that a workgroup takes together: a value that is no number reaches
+    the rows whose tile lists its block, and leaves every other as it was."""
+    n, G = 600, 8
+    q, k, v = rnd(n, 2 * G, 128), rnd(n, 2, 128), rnd(n, 2, 128)
+    lists = _lists([n], [n], 2, False, 1, 64, 5, np.random.default_rng(5))
+    run = lambda vv: bs.block_sparse_attention(q, k, vv, cu([n]), cu([n]), n, lists, block_q=1, causal=True,
+                                               return_lse=True)
+    want, lse = run(v)
+    bad = v.clone()
+    bad[130, 0, 7] = bad[599, 1] = poison
+    out, lse2 = run(bad)
+    assert torch.equal(lse, lse2)
+    hit = torch.zeros(n, 2 * G, 128, dtype=torch.bool, device=DEV)
+    seen = lambda h, j: (lists[:n, h] == j // 64).any(dim=-1) & (torch.arange(n, device=DEV) >= j)
+    hit[seen(0, 130), :G, 7] = True
+    hit[seen(1, 599), G:] = True
+    assert hit.any() and torch.equal(~torch.isfinite(out), hit)
+    assert torch.equal(out[~hit], want[~hit])
 
 
 @pytest.mark.parametrize("bq", [1, 64, 200])
