@@ -675,6 +675,14 @@ template <int D>
 struct RowState {
   f32x16 o[D / 32];
   float m, l;
+  __device__ void reset() {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
+    m = -INFINITY;
+    l = 0.0f;
+  }
 };
 
 // How far (log2) a row's scores may rise above its reference before O is
@@ -684,7 +692,9 @@ constexpr float kSlack = 8.0f;
 
 // One wave's step over NK * 32 keys in LDS (K and V rows from kt / vt): S^T =
 // K Q^T, the probabilities against the row's moving reference, O^T += V^T P^T.
-// The first `keys` keys count (LANES: of each lane's row its own).
+// The first `keys` keys count (LANES: of each lane's row its own; a row of none
+// takes no part: its probabilities are 2^(0 S - inf), which is 0 unless S is no
+// number).
 template <int D, int NK, bool F16, bool LANES = false>
 __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (&qf)[D / 16], int keys, float c,
                                    RowState<D> &st) {
@@ -702,7 +712,7 @@ __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (
       s[kb] = mfma16<F16>(a, qf[x], s[kb]);
     }
   }
-  if (LANES ? __builtin_amdgcn_ballot_w64(keys < 32 * NK) != 0 : keys < 32 * NK) {
+  if (LANES ? __builtin_amdgcn_ballot_w64(keys < 32 * NK && keys > 0) != 0 : keys < 32 * NK) {
     asm volatile("");  // (kept a branch: whole tiles skip the compares)
 #pragma unroll
     for (int kb = 0; kb < NK; ++kb)
@@ -716,6 +726,8 @@ __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (
 #pragma unroll
     for (int i = 0; i < 16; ++i) t = fmaxf(t, s[kb][i]);
   t = both_max(t) * c;
+  const bool none = LANES && keys <= 0;
+  if (none) t = -INFINITY;
   // (the first keys that do not score -inf set the reference)
   const bool raise = t > st.m + kSlack || (st.m == -INFINITY && t > -INFINITY);
   if (__builtin_amdgcn_ballot_w64(raise) != 0) {
@@ -731,13 +743,14 @@ __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (
   // P is rounded to the inputs' 16-bit type for the matrix product (half a unit
   // in the last place of each probability, as O's own rounding); the row sum
   // takes the unrounded ones.
-  const float ref = st.m == -INFINITY ? 0.0f : st.m;
+  const float ref = none ? INFINITY : st.m == -INFINITY ? 0.0f : st.m;
+  const float cl = none ? 0.0f : c;
   typename Elem8<F16>::x8 pb[2 * NK];
 #pragma unroll
   for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -ref));
+      const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][i], cl, -ref));
       st.l += e;
       pb[2 * kb + i / 8][i % 8] = static_cast<typename Elem8<F16>::type>(e);
     }
@@ -759,6 +772,14 @@ struct AttnTile {
   int b, h, q_begin, Lq, tok0, rows;
   TileKeys tk;  // of the last tile
 };
+
+// The item of workgroup i of a causal launch: the tiles with the most keys first,
+// KV heads next to each other (2,047 tokens of 2 KV heads, 16 blocks each: 72 us,
+// 78 in xcd_order's).
+__device__ inline int causal_order(const BlockAttnParams &p, int i) {
+  const int seqs = p.items / p.tiles, tile = i / seqs;
+  return (i - tile * seqs) * p.tiles + (p.tiles - 1 - tile);
+}
 
 // item -> its tile; false where the sequence has no such tile
 __device__ inline bool attn_tile(const BlockAttnParams &p, int item, AttnTile &t) {
@@ -796,6 +817,11 @@ __device__ inline void load_query(const BlockAttnParams &p, const AttnTile &t, i
 // whose keys all score -inf NaN
 __device__ inline float inv_sum(float l, bool keys) { return l > 0.0f || l != l ? 1.0f / l : (keys ? INFINITY : 0.0f); }
 
+// the natural logarithm of a row's softmax sum l against the reference m (log2)
+__device__ inline float log_sum(float m, float l) {
+  return l > 0.0f || l != l ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+}
+
 // O of row r (this lane's), from O^T / l
 template <int D, bool F16>
 __device__ inline void store_rows(const BlockAttnParams &p, const AttnTile &t, int r, const RowState<D> &st, float l,
@@ -815,201 +841,89 @@ __device__ inline void store_rows(const BlockAttnParams &p, const AttnTile &t, i
       for (int e = 0; e < 4; ++e) v[e] = static_cast<typename Elem8<F16>::type>(st.o[db][4 * i + e] * inv);
       *reinterpret_cast<typename Elem8<F16>::x4 *>(o + 32 * db + 8 * i + 4 * hf) = v;
     }
-  if (p.lse && hf == 0)
-    p.lse[static_cast<int64_t>(head) * p.total_q + row] = l > 0.0f || l != l ? (st.m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+  if (p.lse && hf == 0) p.lse[static_cast<int64_t>(head) * p.total_q + row] = log_sum(st.m, l);
 }
 
-// Tiles of up to 32 W rows: W waves of 32 rows, the listed keys in steps of 32
-// through rings of four K and four V tiles in LDS that all waves share, one
-// barrier a step.  Step t computes S(t + 1) = K(t + 1) Q^T beside the
-// exponentials of P(t), independent of each other, then O += V(t)^T P(t); the
-// row maxima of S(t + 1) are taken last, so that the one branch of a step, the
-// rescale of O, lies at its end.  K(t + 4) and V(t + 3) are copied during step t into
-// the slots that step t - 1 was the last to read.
-//
-// What bounds it: a 32-row wave reads 16 KB of LDS fragments for 16 matrix
-// instructions of 32 cycles, which at 128 bytes a cycle for four SIMDs is the
-// same time; two workgroups a compute unit keep both busy.
-template <int N>
-using ic = std::integral_constant<int, N>;
+// The copies of 64 keys' K and V rows into one of two buffers, by W waves
+// together
+template <int D, int W>
+struct TileCopies {
+  static constexpr int ROW = 2 * D, TILE = kSub * ROW;
+  static constexpr int RPC = 64 / (D / 8);       // rows of a copy
+  static constexpr int COPIES = kSub / RPC / W;  // a wave's copies of K, and of V
+  const uint16_t *k, *v;
+  int row_bytes;
+  uint32_t lds;
+  int kvoff[COPIES], vvoff[COPIES];  // this lane's source bytes
+  __device__ TileCopies(const BlockAttnParams &p, const AttnTile &t, char *smem, int wave) {
+    const int64_t off = t.tk.begin * p.kv_tok + (p.per_head ? 0 : t.h * p.kv_head);
+    k = p.k + off;
+    v = p.v + off;
+    row_bytes = static_cast<int>(p.kv_tok) * 2;
+    lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem)) + wave * COPIES * RPC * ROW;
+    const int lane = threadIdx.x & 63, pos = lane % (D / 8);
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int row = (wave * COPIES + i) * RPC + lane / (D / 8);
+      kvoff[i] = row * row_bytes + 16 * k_chunk<D>(row, pos);
+      vvoff[i] = row * row_bytes + 16 * v_chunk<D>(row, pos);
+    }
+  }
+  // keys [key, key + 64) below `limit`
+  __device__ void issue(const BlockAttnParams &p, int key, int buf, int limit) const {
+    const int left = max(0, min(kSub, limit - key));
+    const int64_t off = left > 0 ? key * p.kv_tok : 0;
+    const uint32_t dst = lds + buf * 2 * TILE;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      copy_rows(k + off, static_cast<int64_t>(left) * row_bytes, dst + i * RPC * ROW, kvoff[i]);
+      copy_rows(v + off, static_cast<int64_t>(left) * row_bytes, dst + i * RPC * ROW + TILE, vvoff[i]);
+    }
+  }
+};
 
+// Tiles of up to 32 W rows: W waves of 32 rows, the keys in steps of 64 through
+// two LDS buffers that all waves share.
 template <int D, int W, bool F16>
 __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnParams p) {
-  constexpr int ROW = 2 * D, TILE = 32 * ROW;  // bytes
-  __shared__ __attribute__((aligned(1024))) char smem[8 * TILE];  // four K tiles, four V tiles
-  __shared__ int list[kMaxTopk + 1];
+  constexpr int ROW = 2 * D, TILE = kSub * ROW;  // bytes
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];  // K0 V0 K1 V1
+  __shared__ int list[kMaxTopk + 2];
   __shared__ int scratch[2];
-  const int item = xcd_order(blockIdx.x, p.items);
   AttnTile t;
-  if (!attn_tile(p, item, t)) return;
-  const int lane = threadIdx.x & 63, lq = lane & 31, hf = lane >> 5;
+  if (!attn_tile(p, xcd_order(blockIdx.x, p.items), t)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int blocks = __builtin_amdgcn_readfirstlane(
-      load_list<64 * W>(tile_list(p, t), p.topk, t.tk.blocks, list, scratch));
-  const int n = blocks * (p.bk / 32);  // steps
-  const int r = 32 * wave + lq;
-  const float c = p.scale_log2;
+  const int n = __builtin_amdgcn_readfirstlane(load_list<64 * W>(tile_list(p, t), p.topk, t.tk.blocks, list, scratch));
+  const int r = 32 * wave + (threadIdx.x & 31);
   uint4 qf[D / 16];
   load_query<D>(p, t, r, qf);
   wait_copies<0>();  // (no load of the compiler's own is then pending among the copies)
   RowState<D> st;
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) st.o[db][i] = 0.0f;
-  st.m = -INFINITY;
-  st.l = 0.0f;
-  if (n == 0) {
-    store_rows<D, F16>(p, t, r, st, 0.0f, false);
-    return;
-  }
+  st.reset();
 
-  // ---- copies: a tile's K and V rows are 2 * CP copies of RPC rows each,
-  // PER of them a wave's, all of K or all of V
-  constexpr int RPC = 64 / (D / 8), CP = 32 / RPC, PER = 2 * CP / W;
-  static_assert(PER >= 1 && CP % PER == 0, "copies");
-  const int64_t head_off = p.per_head ? 0 : t.h * p.kv_head;
-  const bool of_v = wave * PER >= CP;
-  const uint16_t *src = (of_v ? p.v : p.k) + t.tk.begin * p.kv_tok + head_off;
-  const int row_bytes = static_cast<int>(p.kv_tok) * 2;
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem)) + (of_v ? 4 * TILE : 0);
-  int voff[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int row = ((wave * PER + i) % CP) * RPC + lane / (D / 8), pos = lane % (D / 8);
-    voff[i] = row * row_bytes + 16 * (of_v ? v_chunk<D>(row, pos) : k_chunk<D>(row, pos));
-  }
-  // a step's first key, its block's end and its place in the list
-  struct Cursor {
-    int key, end, entry, next;  // next: the following block, read a block ahead
-  };
-  auto begin = [&]() {
-    const int key = __builtin_amdgcn_readfirstlane(list[0]) * p.bk;
-    return Cursor{key, key + p.bk, 0, list[1]};
-  };
-  auto advance = [&](Cursor &x) {
-    x.key += 32;
-    if (x.key == x.end) {  // (past the last block the list may hold anything: keys_of has none there)
-      ++x.entry;
-      x.key = __builtin_amdgcn_readfirstlane(x.next) * p.bk;
-      x.end = x.key + p.bk;
-      x.next = list[min(x.entry + 1, kMaxTopk)];
+  const TileCopies<D, W> copies(p, t, smem, wave);
+  int blk = __builtin_amdgcn_readfirstlane(list[0]), off = 0, buf = 0;
+  int nxt = list[1];  // (past the last block it may be anything)
+  if (n > 0) copies.issue(p, blk * p.bk, 0, t.tk.limit);
+  for (int e = 0; e < n;) {
+    const int key = blk * p.bk + off;
+    off += kSub;
+    if (off == p.bk) {
+      off = 0;
+      ++e;
+      blk = __builtin_amdgcn_readfirstlane(nxt);
+      nxt = list[e + 1];
     }
-  };
-  auto keys_of = [&](const Cursor &x) { return x.entry < blocks ? max(0, t.tk.limit - x.key) : 0; };
-  Cursor copied = begin(), masked = begin();
-  auto copy = [&](auto slot) {
-    const int left = min(32, keys_of(copied));
-    const int64_t off = left > 0 ? copied.key * p.kv_tok : 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      copy_rows(src + off, static_cast<int64_t>(left) * row_bytes,
-                lds0 + (decltype(slot)::value & 3) * TILE + ((wave * PER + i) % CP) * RPC * ROW, voff[i]);
-    advance(copied);
-  };
-
-  // ---- fragment addresses
-  int kaddr[D / 16], vaddr[D / 32];
-#pragma unroll
-  for (int x = 0; x < D / 16; ++x) kaddr[x] = lq * ROW + 16 * k_chunk<D>(lq, 2 * x + hf);
-  const int vr = 4 * hf + ((lane & 15) >> 2), vc = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db) vaddr[db] = vr * ROW + 16 * v_chunk<D>(vr, 4 * db + vc / 8) + 2 * (vc % 8);
-  auto scores = [&](auto slot, f32x16 &s) {
-    uint4 kf[D / 16];
-#pragma unroll
-    for (int x = 0; x < D / 16; ++x)
-      kf[x] = *reinterpret_cast<const uint4 *>(smem + (decltype(slot)::value & 3) * TILE + kaddr[x]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-    for (int x = 0; x < D / 16; ++x) s = mfma16<F16>(kf[x], qf[x], s);
-  };
-  // the keys past `keys` out, and the reference raised where a score is far above it
-  auto settle = [&](f32x16 &s, int keys) {
-    if (keys < 32) {
-      asm volatile("");  // (kept a branch: whole tiles skip the compares)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (8 * (i / 4) + 4 * hf + i % 4 >= keys) s[i] = -INFINITY;
-    }
-    float x = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) x = fmaxf(x, s[i]);
-    x = both_max(x) * c;
-    const bool raise = x > st.m + kSlack || (st.m == -INFINITY && x > -INFINITY);
-    if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-      const float f = raise ? __builtin_amdgcn_exp2f(st.m - x) : 1.0f;
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st.o[db][i] *= f;
-      st.l *= f;
-      st.m = raise ? x : st.m;
-    }
-  };
-  f32x16 sa, sb;
-  auto step = [&](auto tt) {
-    constexpr int T = decltype(tt)::value;
-    f32x16 &cur = T & 1 ? sb : sa;
-    f32x16 &nxt = T & 1 ? sa : sb;
-    scores(ic<T + 1>(), nxt);
-    const float ref = st.m == -INFINITY ? 0.0f : st.m;
-    typename Elem8<F16>::x8 pb[2];
-    float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float e = __builtin_amdgcn_exp2f(fmaf(cur[i], c, -ref));
-      (i & 1 ? l1 : l0) += e;
-      pb[i / 8][i % 8] = static_cast<typename Elem8<F16>::type>(e);
-    }
-    st.l += l0 + l1;
-    const char *vt = smem + (4 + T) * TILE;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db) {
-        const char *p0 = vt + vaddr[db] + 16 * ks * ROW;
-        const i16x4 a8[2] = {lds_read_tr(p0), lds_read_tr(p0 + 8 * ROW)};  // (rows 8 apart lie alike)
-        st.o[db] = mfma16<F16>(__builtin_bit_cast(uint4, a8), __builtin_bit_cast(uint4, pb[ks]), st.o[db]);
-      }
-    settle(nxt, keys_of(masked));
-    advance(masked);
-  };
-  // two steps, T and T + 1, between barriers: what they read has arrived, and
-  // the slots that the two before read are free
-  auto turn = [&](auto tt) {
-    constexpr int T = decltype(tt)::value;
     wait_copies<0>();
     wait_reads();
-    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_s_barrier();  // the step has arrived, and no wave reads the other buffer any more
     asm volatile("" ::: "memory");
-    if (of_v) {
-      copy(ic<T + 2>());
-      copy(ic<T + 3>());
-    } else {
-      copy(ic<T + 3>());
-      copy(ic<T>());
-    }
-    step(ic<T>());
-    step(ic<T + 1>());
-  };
-  // K(0 .. 2) and V(0 .. 1)
-  copy(ic<0>());
-  copy(ic<1>());
-  if (!of_v) copy(ic<2>());
-  wait_copies<0>();
-  __syncthreads();
-  scores(ic<0>(), sa);
-  settle(sa, keys_of(masked));
-  advance(masked);
-  // whole turns of the rings: steps past the last copy zeros and mask every key
-  for (int s = 0; s < n; s += 4) {
-    turn(ic<0>());
-    turn(ic<2>());
+    if (e < n) copies.issue(p, blk * p.bk + off, buf ^ 1, t.tk.limit);
+    const char *kt = smem + buf * 2 * TILE;
+    attend_step<D, 2, F16>(kt, kt + TILE, qf, max(0, t.tk.limit - key), p.scale_log2, st);
+    buf ^= 1;
   }
-  wait_copies<0>();  // no copy may land in LDS after the workgroup ends
-  store_rows<D, F16>(p, t, r, st, both_sum(st.l), true);
+  store_rows<D, F16>(p, t, r, st, both_sum(st.l), n > 0);
 }
 
 // Several consecutive small tiles at once (a prompt in which every token has a
@@ -1024,74 +938,26 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
 // one instead.
 constexpr int kWindow = 1024;    // blocks whose lists are joined at a time
 constexpr int kMaxGroup = 32;    // tiles: a bit each
-constexpr int kGroupItems = 256; // workgroups that a launch in groups has at least
+constexpr int kGroupItems = 128; // workgroups that a launch in groups has at least
 
 template <int D, int W, bool F16>
 __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnParams p) {
   constexpr int ROW = 2 * D, TILE = kSub * ROW;  // bytes
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];  // K0 V0 K1 V1
-  __shared__ int list[kWindow];
-  __shared__ uint32_t members[kWindow];  // of the window's blocks, the tiles that list them
+  __shared__ int list[kWindow + 2];      // the window's blocks that any tile lists, in order
+  __shared__ uint32_t members[kWindow];  // of every block of the window, the tiles that list it
   __shared__ int scratch[W > 2 ? W : 2];
   static_assert(kWindow % (64 * W) == 0, "window");
-  const int item = xcd_order(blockIdx.x, p.items);
   AttnTile t;
-  if (!attn_tile(p, item, t)) return;
+  if (!attn_tile(p, p.causal ? causal_order(p, blockIdx.x) : xcd_order(blockIdx.x, p.items), t)) return;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = p.bk / kSub;
-
   const int r = 32 * wave + (lane & 31);
   uint4 qf[D / 16];
   load_query<D>(p, t, r, qf);
   wait_copies<0>();  // (no load of the compiler's own is then pending among the copies)
-  RowState<D> st;
 
-  const int64_t head_off = p.per_head ? 0 : t.h * p.kv_head;
-  const uint16_t *kp = p.k + t.tk.begin * p.kv_tok + head_off;
-  const uint16_t *vp = p.v + t.tk.begin * p.kv_tok + head_off;
-  constexpr int RPC = 64 / (D / 8);          // rows of a copy
-  constexpr int COPIES = kSub / RPC / W;     // a wave's copies of K, and of V, per step
-  const int crow = lane / (D / 8), cpos = lane % (D / 8);
-  const int row_bytes = static_cast<int>(p.kv_tok) * 2;
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem));
-  auto block_of = [&](int s) { return __builtin_amdgcn_readfirstlane(list[s / per]); };
-  auto first_key = [&](int s) { return block_of(s) * p.bk + (s % per) * kSub; };
-  auto issue = [&](int s, int buf, int limit) {
-    const int key = first_key(s);
-    const int64_t left = max(0, min(kSub, limit - key));
-    const int64_t off = left > 0 ? key * p.kv_tok : 0;
-    const uint32_t dst = lds0 + buf * 2 * TILE;
-#pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      const int row = (wave * COPIES + i) * RPC + crow;
-      const uint32_t at = dst + (wave * COPIES + i) * RPC * ROW;
-      copy_rows(kp + off, left * row_bytes, at, row * row_bytes + 16 * k_chunk<D>(row, cpos));
-      copy_rows(vp + off, left * row_bytes, at + TILE, row * row_bytes + 16 * v_chunk<D>(row, cpos));
-    }
-  };
-  auto reset = [&]() {
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st.o[db][i] = 0.0f;
-    st.m = -INFINITY;
-    st.l = 0.0f;
-  };
-  // the steps of list[0 .. n / per), keys up to `limit`; step(s, tile in LDS)
-  auto walk = [&](int n, int limit, auto &&step) {
-    if (n > 0) issue(0, 0, limit);
-    for (int s = 0; s < n; ++s) {
-      wait_copies<0>();
-      wait_reads();
-      __builtin_amdgcn_s_barrier();  // step s has arrived, and no wave reads the other buffer any more
-      asm volatile("" ::: "memory");
-      if (s + 1 < n) issue(s + 1, (s + 1) & 1, limit);
-      step(s, smem + (s & 1) * 2 * TILE);
-    }
-  };
-  reset();
-
+  const TileCopies<D, W> copies(p, t, smem, wave);
   const int32_t *src = tile_list(p, t);
   const int64_t row = static_cast<int64_t>(p.Hkv) * p.topk;
   const int last = (t.rows / p.G - 1) / p.bq;  // the group's last tile, whose limit t.tk has
@@ -1104,9 +970,13 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnPa
     const int lo = 32 * wave / p.G / p.bq, hi = min(32 * wave + 31, t.rows - 1) / p.G / p.bq;
     wave_tiles = (0xffffffffu >> (31 - (hi - lo))) << lo;
   }
-  bool seen = false;  // whether this lane's row had a key
-  // walks the union of the lists, or tile `only`'s
-  auto pass = [&](int only) {
+  wave_tiles = __builtin_amdgcn_readfirstlane(wave_tiles);
+
+  // the union of the lists (only < 0), and only if that will not do each tile's
+  for (int only = -1; only <= last; ++only) {
+    RowState<D> st;
+    st.reset();
+    bool seen = false;  // whether this lane's row had a key
     const int limit = only < 0 ? t.tk.limit : limit_of(only);
     const uint32_t take = only < 0 ? 0xffffffffu : 1u << only;
     for (int w0 = 0; w0 < t.tk.blocks; w0 += kWindow) {
@@ -1120,7 +990,7 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnPa
           atomicOr(&members[x - w0], (1u << tile) & take);
       }
       __syncthreads();
-      // the blocks that any tile lists, in order: each thread a run of them
+      // each thread a run of the window
       constexpr int RUN = kWindow / (64 * W);
       int mine = 0;
 #pragma unroll
@@ -1139,38 +1009,50 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnPa
         if (members[threadIdx.x * RUN + i] != 0) list[at++] = w0 + threadIdx.x * RUN + i;
       __syncthreads();
       n = __builtin_amdgcn_readfirstlane(n);
-      walk(n * per, limit, [&](int s, const char *kt) {
-        const int blk = block_of(s);
-        const uint32_t who = __builtin_amdgcn_readfirstlane(members[blk - w0]);
-        if ((who & wave_tiles) == 0) return;
-        const int keys = (who >> my_tile) & 1 ? max(0, my_limit - first_key(s)) : 0;
-        seen = seen || keys > 0;
-        attend_step<D, 2, F16, true>(kt, kt + TILE, qf, keys, p.scale_log2, st);
-      });
+      if (n == 0) continue;
+
+      int blk = __builtin_amdgcn_readfirstlane(list[0]), off = 0, buf = 0;
+      int nxt = list[1];  // (past the last block it may be anything)
+      copies.issue(p, blk * p.bk, 0, limit);
+      for (int e = 0; e < n;) {
+        const int key = blk * p.bk + off;
+        const uint32_t who_v = members[blk - w0];
+        off += kSub;
+        if (off == p.bk) {
+          off = 0;
+          ++e;
+          blk = __builtin_amdgcn_readfirstlane(nxt);
+          nxt = list[e + 1];
+        }
+        wait_copies<0>();
+        wait_reads();
+        __builtin_amdgcn_s_barrier();  // the step has arrived, and no wave reads the other buffer any more
+        asm volatile("" ::: "memory");
+        if (e < n) copies.issue(p, blk * p.bk + off, buf ^ 1, limit);
+        const uint32_t who = __builtin_amdgcn_readfirstlane(who_v);
+        if ((who & wave_tiles) != 0) {
+          const char *kt = smem + buf * 2 * TILE;
+          const int keys = (who >> my_tile) & 1 ? max(0, my_limit - key) : 0;
+          seen = seen || keys > 0;
+          attend_step<D, 2, F16, true>(kt, kt + TILE, qf, keys, p.scale_log2, st);
+        }
+        buf ^= 1;
+      }
     }
-  };
-  pass(-1);
-  float check = st.l;
+    if (only >= 0) {
+      store_rows<D, F16>(p, t, my_tile == only ? r : t.rows, st, both_sum(st.l), seen);
+      continue;
+    }
+    float check = st.l;
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
+    for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) check = fmaf(st.o[db][i], 0.0f, check);
-  const bool odd = __builtin_amdgcn_ballot_w64(r < t.rows && !(check - check == 0.0f)) != 0;
-  __syncthreads();
-  if (threadIdx.x == 0) scratch[0] = 0;
-  __syncthreads();
-  if (odd && lane == 0) scratch[0] = 1;
-  __syncthreads();
-  const bool again = __builtin_amdgcn_readfirstlane(scratch[0]) != 0;
-  if (!again) {
-    store_rows<D, F16>(p, t, r, st, both_sum(st.l), seen);
-    return;
-  }
-  for (int tile = 0; tile <= last; ++tile) {
-    reset();
-    seen = false;
-    pass(tile);
-    store_rows<D, F16>(p, t, my_tile == tile ? r : t.rows, st, both_sum(st.l), seen);
+      for (int i = 0; i < 16; ++i) check = fmaf(st.o[db][i], 0.0f, check);
+    const bool odd = __builtin_amdgcn_ballot_w64(r < t.rows && !(check - check == 0.0f)) != 0;
+    if (!__syncthreads_or(odd)) {
+      store_rows<D, F16>(p, t, r, st, both_sum(st.l), seen);
+      return;
+    }
   }
 }
 
@@ -1200,63 +1082,80 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
   if (!attn_tile(p, item, t)) return;
   const int lane = threadIdx.x & 63, lq = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = p.bk / 32;
-  const int n = __builtin_amdgcn_readfirstlane(
-                    load_list<64 * kSmallWaves>(tile_list(p, t), p.topk, t.tk.blocks, list, scratch)) * per;
-
+  const int32_t *src = tile_list(p, t);
   uint4 qf[D / 16];
   load_query<D>(p, t, lq, qf);
-  wait_copies<0>();
+  // a list that fits the lanes, ascending and then none, stays in them
+  const int x = lane < p.topk ? src[lane] : -1;
+  const bool valid = x >= 0 && x < t.tk.blocks;
+  const uint64_t valids = __builtin_amdgcn_ballot_w64(valid);
+  const int before = __shfl_up(x, 1);  // (by every lane: one that did not take part has nothing to read from)
+  const bool odd = valid && lane > 0 && !((valids >> (lane - 1) & 1) && before < x);
+  const bool in_lanes = p.topk <= 64 && __builtin_amdgcn_ballot_w64(odd) == 0;
+  const int n = in_lanes ? __popcll(valids)
+                         : __builtin_amdgcn_readfirstlane(
+                               load_list<64 * kSmallWaves>(src, p.topk, t.tk.blocks, list, scratch));
+  auto block = [&](int e) {
+    return in_lanes ? __builtin_amdgcn_readlane(x, e) : __builtin_amdgcn_readfirstlane(list[e]);
+  };
+  wait_copies<0>();  // (no load of the compiler's own is then pending among the copies)
   RowState<D> st;
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) st.o[db][i] = 0.0f;
-  st.m = -INFINITY;
-  st.l = 0.0f;
+  st.reset();
 
-  const int64_t head_off = p.per_head ? 0 : t.h * p.kv_head;
-  const uint16_t *kp = p.k + t.tk.begin * p.kv_tok + head_off;
-  const uint16_t *vp = p.v + t.tk.begin * p.kv_tok + head_off;
+  const int64_t head_off = t.tk.begin * p.kv_tok + (p.per_head ? 0 : t.h * p.kv_head);
+  const uint16_t *kp = p.k + head_off, *vp = p.v + head_off;
   constexpr int RPC = 64 / (D / 8), COPIES = 32 / RPC;  // copies of K, and of V, per step
-  const int crow = lane / (D / 8), cpos = lane % (D / 8);
   const int row_bytes = static_cast<int>(p.kv_tok) * 2;
   char *ring = smem + wave * kRing * 2 * TILE;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)ring));
-  auto first_key = [&](int s) {
-    const int blk = __builtin_amdgcn_readfirstlane(list[s / per]);
-    return blk * p.bk + (s % per) * 32;
-  };
-  auto issue = [&](int s, int buf) {
-    const int key = first_key(s);
-    const int64_t left = max(0, min(32, t.tk.limit - key));
+  int kvoff[COPIES], vvoff[COPIES];
+#pragma unroll
+  for (int i = 0; i < COPIES; ++i) {
+    const int row = i * RPC + lane / (D / 8), pos = lane % (D / 8);
+    kvoff[i] = row * row_bytes + 16 * k_chunk<D>(row, pos);
+    vvoff[i] = row * row_bytes + 16 * v_chunk<D>(row, pos);
+  }
+  auto issue = [&](int key, int buf) {
+    const int left = max(0, min(32, t.tk.limit - key));
     const int64_t off = left > 0 ? key * p.kv_tok : 0;
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
-      const int row = i * RPC + crow;
       const uint32_t at = lds0 + buf * 2 * TILE + i * RPC * ROW;
-      copy_rows(kp + off, left * row_bytes, at, row * row_bytes + 16 * k_chunk<D>(row, cpos));
-      copy_rows(vp + off, left * row_bytes, at + TILE, row * row_bytes + 16 * v_chunk<D>(row, cpos));
+      copy_rows(kp + off, static_cast<int64_t>(left) * row_bytes, at, kvoff[i]);
+      copy_rows(vp + off, static_cast<int64_t>(left) * row_bytes, at + TILE, vvoff[i]);
     }
   };
-  const int step = kSmallWaves * p.splits;
-  int s = wave * p.splits + split;
-  if (s < n) issue(s, 0);
-  for (int it = 0; s < n; s += step, ++it) {
+  // this wave's steps: every (4 * splits)-th 32 keys of the list, as an entry and an
+  // offset in its block
+  const int stride = 32 * kSmallWaves * p.splits, blocks_on = stride / p.bk, keys_on = stride - blocks_on * p.bk;
+  const int start = 32 * (wave * p.splits + split);
+  int e = start / p.bk, off = start - e * p.bk;
+  int key = e < n ? block(e) * p.bk + off : 0;
+  if (e < n) issue(key, 0);
+  for (int buf = 0; e < n; buf ^= 1) {
+    const int now = key;
+    e += blocks_on;
+    off += keys_on;
+    if (off >= p.bk) {
+      off -= p.bk;
+      ++e;
+    }
     wait_reads();  // the other buffer has been read
-    if (s + step < n) {
-      issue(s + step, (it + 1) & 1);
+    if (e < n) {
+      key = block(e) * p.bk + off;
+      issue(key, buf ^ 1);
       wait_copies<2 * COPIES>();
     } else {
       wait_copies<0>();
     }
     asm volatile("" ::: "memory");
-    const char *kt = ring + (it & 1) * 2 * TILE;
-    attend_step<D, 1, F16>(kt, kt + TILE, qf, max(0, t.tk.limit - first_key(s)), p.scale_log2, st);
+    const char *kt = ring + buf * 2 * TILE;
+    attend_step<D, 1, F16>(kt, kt + TILE, qf, max(0, t.tk.limit - now), p.scale_log2, st);
   }
   const float l = both_sum(st.l);
 
   // joined: the waves' O^T in LDS, scaled to the largest reference
+  const bool here = lq < t.rows;
   __syncthreads();
   if (hf == 0) ml[wave][lq] = make_float2(st.m, l);
   __syncthreads();
@@ -1267,22 +1166,23 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
   float sum = 0.0f;
 #pragma unroll
   for (int w = 0; w < kSmallWaves; ++w) {
-    const float2 x = ml[w][lq];
-    sum += x.y == 0.0f ? 0.0f : x.y * __builtin_amdgcn_exp2f(x.x - ref);
+    const float2 y = ml[w][lq];
+    sum += y.y == 0.0f ? 0.0f : y.y * __builtin_amdgcn_exp2f(y.x - ref);
   }
   const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(st.m - ref);
   float4 *buf = reinterpret_cast<float4 *>(smem);  // [wave][register quad][lane]
   constexpr int QUADS = D / 8;
+  if (here)
 #pragma unroll
-  for (int i = 0; i < QUADS; ++i) {
-    const f32x16 &o = st.o[i / 4];
-    const int e = 4 * (i % 4);
-    buf[(wave * QUADS + i) * 64 + lane] = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
-  }
+    for (int i = 0; i < QUADS; ++i) {
+      const f32x16 &o = st.o[i / 4];
+      const int q = 4 * (i % 4);
+      buf[(wave * QUADS + i) * 64 + lane] = make_float4(o[q] * f, o[q + 1] * f, o[q + 2] * f, o[q + 3] * f);
+    }
   __syncthreads();
+  if (!here) return;
   const int tok = lq / p.G, g = lq - tok * p.G, head = t.h * p.G + g;
   const int64_t row = t.q_begin + static_cast<int64_t>(t.tok0) + tok;
-  const bool here = lq < t.rows;
   const float inv = inv_sum(sum, n > 0);
   float *part = p.part + (static_cast<int64_t>(item) * p.splits + split) * PartLayout<D>::kFloats + lq * PartLayout<D>::kRow;
 #pragma unroll
@@ -1290,11 +1190,10 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
     float4 a = buf[i * 64 + lane];
 #pragma unroll
     for (int w = 1; w < kSmallWaves; ++w) {
-      const float4 x = buf[(w * QUADS + i) * 64 + lane];
-      a = make_float4(a.x + x.x, a.y + x.y, a.z + x.z, a.w + x.w);
+      const float4 y = buf[(w * QUADS + i) * 64 + lane];
+      a = make_float4(a.x + y.x, a.y + y.y, a.z + y.z, a.w + y.w);
     }
     const int d = 8 * i + 4 * hf;
-    if (!here) continue;
     if (p.splits > 1) {
       *reinterpret_cast<float4 *>(part + d) = a;
     } else {
@@ -1306,19 +1205,20 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
       *reinterpret_cast<typename Elem8<F16>::x4 *>(p.o + row * p.o_tok + head * p.o_head + d) = v;
     }
   }
-  if (!here || wave != 0 || hf != 0) return;
+  if (wave != 0 || hf != 0) return;
   if (p.splits > 1) {
     *reinterpret_cast<float4 *>(part + D) = make_float4(m, sum, n > 0 ? 1.0f : 0.0f, 0.0f);
   } else if (p.lse) {
-    p.lse[static_cast<int64_t>(head) * p.total_q + row] =
-        sum > 0.0f || sum != sum ? (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -INFINITY;
+    p.lse[static_cast<int64_t>(head) * p.total_q + row] = log_sum(m, sum);
   }
 }
 
-// The parts of a tile's workgroups, added up in their order: one wave per
-// query row, lane i columns i, i + 64.
+// The parts of a tile's workgroups, added up in their order: one wave per query
+// row.  Lane i first holds part i's reference and sum (64 parts at a time), then
+// columns i and i + 64; parts are read eight together.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) block_attn_join_kernel(BlockAttnParams p) {
+  constexpr int FLOATS = PartLayout<D>::kFloats, C = D / 64, kAhead = 8;
   const int rows = p.bq * p.G;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int item = static_cast<int>(w / rows), r = static_cast<int>(w - static_cast<int64_t>(item) * rows);
@@ -1326,32 +1226,54 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(BlockAttnParams p)
   AttnTile t;
   if (!attn_tile(p, item, t) || r >= t.rows) return;
   const int lane = threadIdx.x & 63;
-  const float *part = p.part + static_cast<int64_t>(item) * p.splits * PartLayout<D>::kFloats + r * PartLayout<D>::kRow;
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, part[s * PartLayout<D>::kFloats + D]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f, o[D / 64];
+  const float *part = p.part + static_cast<int64_t>(item) * p.splits * FLOATS + r * PartLayout<D>::kRow;
+  float m = -INFINITY, sum = 0.0f, o[C];
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) o[i] = 0.0f;
+  for (int c = 0; c < C; ++c) o[c] = 0.0f;
   bool keys = false;
-  for (int s = 0; s < p.splits; ++s) {
-    const float *x = part + s * PartLayout<D>::kFloats;
-    const float l = x[D + 1], f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[D] - ref);
-    sum += l * f;
-    keys = keys || x[D + 2] != 0.0f;
+  for (int s0 = 0; s0 < p.splits; s0 += 64) {
+    const int cnt = min(64, p.splits - s0);
+    const float *x = part + static_cast<int64_t>(s0) * FLOATS;
+    const float4 mine = lane < cnt ? *reinterpret_cast<const float4 *>(x + static_cast<int64_t>(lane) * FLOATS + D)
+                                   : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    float top = mine.x, add;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] += x[64 * i + lane] * f;
+    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    top = fmaxf(top, m);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    const float f = mine.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mine.x - ref);
+    const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - ref);
+    add = mine.y * f;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) add += __shfl_xor(add, off);
+    sum = sum * old + add;
+    keys = keys || __builtin_amdgcn_ballot_w64(mine.z != 0.0f) != 0;
+    m = top;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] *= old;
+    for (int s = 0; s < cnt; s += kAhead) {
+      float v[kAhead][C];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[i][c] = x[static_cast<int64_t>(min(s + i, cnt - 1)) * FLOATS + 64 * c + lane];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float fi = __shfl(f, s + i);  // (0 past the last part)
+        if (s + i < cnt)
+#pragma unroll
+          for (int c = 0; c < C; ++c) o[c] = fmaf(v[i][c], fi, o[c]);
+      }
+    }
   }
   const int tok = r / p.G, g = r - tok * p.G, head = t.h * p.G + g;
   const int64_t row = t.q_begin + static_cast<int64_t>(t.tok0) + tok;
   const float inv = inv_sum(sum, keys);
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-    p.o[row * p.o_tok + head * p.o_head + 64 * i + lane] =
-        __builtin_bit_cast(uint16_t, static_cast<typename Elem8<F16>::type>(o[i] * inv));
-  if (p.lse && lane == 0)
-    p.lse[static_cast<int64_t>(head) * p.total_q + row] =
-        sum > 0.0f || sum != sum ? (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -INFINITY;
+  for (int c = 0; c < C; ++c)
+    p.o[row * p.o_tok + head * p.o_head + 64 * c + lane] =
+        __builtin_bit_cast(uint16_t, static_cast<typename Elem8<F16>::type>(o[c] * inv));
+  if (p.lse && lane == 0) p.lse[static_cast<int64_t>(head) * p.total_q + row] = log_sum(m, sum);
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -1609,12 +1531,14 @@ static AttnPlan attn_plan(const pkv_block_attn_args *a) {
   s.tiles = (tiles + s.group - 1) / s.group;
   s.items = heads * s.tiles;
   if (rows <= 32 && s.group == 1 && s.items > 0) {
-    // as many workgroups as give the chip one each, but at least four 32-key
-    // steps a wave
+    // as many workgroups as give the chip one each, at least one 32-key step a
+    // wave, where a workgroup alone would take eight: joining the parts costs
+    // what four steps do (8 tiles of 32 blocks 13.0 us in 16 parts, 15.0 in 4; 2
+    // tiles of 8 blocks 10.1 alone, 12.6 in 4)
     int64_t n = 256 / s.items;
-    const int64_t most = static_cast<int64_t>(a->topk) * (a->block_k / 32) / (4 * kSmallWaves);
-    if (n > most) n = most;
-    if (n > 1) s.splits = static_cast<int>(n);
+    const int64_t steps = static_cast<int64_t>(a->topk) * (a->block_k / 32) / kSmallWaves;
+    if (n > steps) n = steps;
+    if (steps >= 8 && n > 1) s.splits = static_cast<int>(n);
   }
   return s;
 }
