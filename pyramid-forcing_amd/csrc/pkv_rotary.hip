@@ -40,7 +40,7 @@ struct RotParams {
   void *qo, *ko;
   const void *pos;
   const double *freqs;
-  int64_t rows;
+  int64_t row0, rows;  // this launch's first row; the rows of all
   int64_t q_tok, q_head, k_tok, k_head, pos_row;
   int Hq, heads, D, pairs, n_axes, tokens;
   int axis_end[PKV_ROTARY_MAX_AXES];
@@ -73,7 +73,7 @@ struct RotVec<T, 1> {
 template <typename T, int V, bool HALF>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotParams p) {
   extern __shared__ float2 cs[];  // [tokens][pairs]: cosine and sine, scaled
-  const int64_t tok0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
+  const int64_t tok0 = p.row0 + static_cast<int64_t>(blockIdx.x) * p.tokens;
   const int left = p.rows - tok0 < p.tokens ? static_cast<int>(p.rows - tok0) : p.tokens;
   for (int e = threadIdx.x; e < left * p.pairs; e += kRotThreads) {
     const int t = div_by(e, p.by_pairs), j = e - t * p.pairs;
@@ -155,16 +155,20 @@ static int launch_rotary(const pkv_rotary_args *a, RotParams &p, hipStream_t st)
   const int V = !vec ? 1 : a->interleaved ? W / 2 : W;
   const int E = !vec ? (a->interleaved ? 2 : 1) : W;
   p.by_items = fast_div(p.pairs / V + (p.D - 2 * p.pairs) / E);
-  const int64_t grid = (p.rows + p.tokens - 1) / p.tokens;
-  if (grid > 0x7fffffff) return fail(PKV_ERR_UNSUPPORTED, "rotary: too many rows");
   void (*k)(RotParams) = nullptr;
   if (a->interleaved)
     k = vec ? rotary_kernel<T, W / 2, false> : rotary_kernel<T, 1, false>;
   else
     k = vec ? rotary_kernel<T, W, true> : rotary_kernel<T, 1, true>;
-  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(kRotThreads), sizeof(float2) * p.tokens * p.pairs, st,
-                     p);
-  return check_launch("rotary_kernel");
+  // a launch counts its threads in 32 bits
+  constexpr int64_t kMost = 0xffffffffll / kRotThreads;
+  for (; p.row0 < p.rows; p.row0 += kMost * p.tokens) {
+    const int64_t left = (p.rows - p.row0 + p.tokens - 1) / p.tokens;
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(left < kMost ? left : kMost)), dim3(kRotThreads),
+                       sizeof(float2) * p.tokens * p.pairs, st, p);
+    if (const int rc = check_launch("rotary_kernel")) return rc;
+  }
+  return PKV_OK;
 }
 
 }  // namespace pkv

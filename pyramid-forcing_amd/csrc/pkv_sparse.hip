@@ -68,12 +68,13 @@ struct MeansParams {
   int64_t total_rows;
   int64_t tok, head;
   int S, H, bk, last, total_k;
+  int chunks;  // workgroups of a sequence
 };
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) block_means_kernel(MeansParams p) {
   constexpr int LPR = D / 8, RPI = 64 / LPR;  // lanes of a key row, rows of a read
-  const int s = blockIdx.y;
+  const int s = blockIdx.x / p.chunks, chunk = blockIdx.x - s * p.chunks;
   const Span keys = key_span(p.cu, p.used, s, p.total_k);
   const int begin = keys.begin, n = keys.n;
   const int64_t first = begin / p.bk + s;
@@ -82,8 +83,8 @@ __global__ void __launch_bounds__(256) block_means_kernel(MeansParams p) {
   const int from = p.last > 0 ? max(0, n - p.last) / p.bk : 0;
   const int64_t to = p.last > 0 ? (n + p.bk - 1) / p.bk : end - first;
   const int lane = threadIdx.x & 63, col = 8 * (lane % LPR), sub = lane / LPR;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * 4;
-  for (int64_t w = static_cast<int64_t>(from) * p.H + blockIdx.x * 4 + (threadIdx.x >> 6); w < to * p.H; w += stride) {
+  const int64_t stride = static_cast<int64_t>(p.chunks) * 4;
+  for (int64_t w = static_cast<int64_t>(from) * p.H + chunk * 4 + (threadIdx.x >> 6); w < to * p.H; w += stride) {
     const int64_t j = w / p.H;
     const int h = static_cast<int>(w - j * p.H);
     const int64_t left = n - j * p.bk;
@@ -1259,7 +1260,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(BlockAttnParams p)
         for (int c = 0; c < C; ++c) v[i][c] = x[static_cast<int64_t>(min(s + i, cnt - 1)) * FLOATS + 64 * c + lane];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const float fi = __shfl(f, s + i);  // (0 past the last part)
+        const float fi = __shfl(f, s + i);
         if (s + i < cnt)
 #pragma unroll
           for (int c = 0; c < C; ++c) o[c] = fmaf(v[i][c], fi, o[c]);
@@ -1277,6 +1278,10 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(BlockAttnParams p)
 }
 
 // ---- host ------------------------------------------------------------------------
+// threads that a launch has at most in a dimension: the dispatch counts them in
+// 32 bits
+constexpr int64_t kMaxThreads = 0xffffffffll;
+
 // cu_seqlens are 32-bit: rows past them belong to no sequence
 static int row_count(int64_t n) { return n < 0x7fffffff ? static_cast<int>(n) : 0x7fffffff; }
 
@@ -1315,23 +1320,26 @@ extern "C" int pkv_block_means(const pkv_block_means_args *a, pkv_stream_t strea
     return fail(PKV_ERR_INVALID, "block_means: NULL argument");
   if ((a->kv_tok_stride | a->kv_head_stride) & 7)
     return fail(PKV_ERR_INVALID, "block_means: strides must keep 16-byte rows aligned");
-  if (a->num_seqs > 65535) return fail(PKV_ERR_UNSUPPORTED, "block_means: %d sequences (at most 65535)", a->num_seqs);
+  if (a->num_seqs > kMaxThreads / 256) return fail(PKV_ERR_UNSUPPORTED, "block_means: too many sequences");
   MeansParams p{};
   p.k = a->k; p.means = a->means; p.cu = a->cu_seqlens_k; p.used = a->seqlens_k;
   p.total_rows = a->total_k / a->block_k + a->num_seqs;
   p.tok = a->kv_tok_stride; p.head = a->kv_head_stride;
   p.S = a->num_seqs; p.H = a->num_heads; p.bk = a->block_k; p.last = a->last;
   p.total_k = row_count(a->total_k);
-  // a wave per block and head of a sequence of the bound's length (longer ones loop)
+  // a wave per block and head of a sequence of the bound's length, as long as
+  // those make no more workgroups than fill the chip many times (the others loop)
   const int64_t longest = a->max_seqlen_k > 0 ? a->max_seqlen_k : a->total_k;
   int64_t blocks = a->last > 0 ? a->last / a->block_k + 2 : longest / a->block_k + 1;
   if (blocks > longest / a->block_k + 1) blocks = longest / a->block_k + 1;
-  int64_t grid = (blocks * a->num_heads + 3) / 4;
-  if (grid > 65536) grid = 65536;
+  int64_t chunks = (blocks * a->num_heads + 3) / 4;
+  const int64_t most = 65536 / a->num_seqs;
+  if (chunks > most) chunks = most > 1 ? most : 1;
+  p.chunks = static_cast<int>(chunks);
   const bool f16 = a->dtype == PKV_DTYPE_FP16;
   auto *k = a->head_dim == 128 ? (f16 ? block_means_kernel<128, true> : block_means_kernel<128, false>)
                                : (f16 ? block_means_kernel<64, true> : block_means_kernel<64, false>);
-  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid), a->num_seqs), dim3(256), 0, as_stream(stream), p);
+  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(a->num_seqs * chunks)), dim3(256), 0, as_stream(stream), p);
   return check_launch("block_means_kernel");
 }
 
@@ -1503,7 +1511,7 @@ static int check_attn(const pkv_block_attn_args *a) {
     return fail(PKV_ERR_INVALID, "block_attn: softmax_scale must be above 0 and finite");
   const int64_t items = static_cast<int64_t>(a->num_batches) * a->num_heads_kv *
                         ((static_cast<int64_t>(a->max_seqlen_q) + a->block_q - 1) / a->block_q);
-  if (items > 0x1fffffff || a->total_q > 0x7fffffff) return fail(PKV_ERR_UNSUPPORTED, "block_attn: grid too large");
+  if (items > kMaxThreads / 512 || a->total_q > 0x7fffffff) return fail(PKV_ERR_UNSUPPORTED, "block_attn: grid too large");
   return PKV_OK;
 }
 
@@ -1583,9 +1591,11 @@ extern "C" int pkv_block_attn(const pkv_block_attn_args *a, void *workspace, int
   if (((a->q_tok_stride | a->q_head_stride | a->kv_tok_stride | a->kv_head_stride) & 7) ||
       ((a->o_tok_stride | a->o_head_stride) & 3))
     return fail(PKV_ERR_INVALID, "block_attn: strides must keep 16-byte rows aligned");
-  // buffer offsets within one step of keys are 32-bit
-  if (a->kv_tok_stride < 0 || a->kv_tok_stride * 2 * kSub > 0x7fffffff)
-    return fail(PKV_ERR_UNSUPPORTED, "block_attn: kv token stride too large");
+  // buffer offsets within one step of keys are 32-bit; a step's bound is its keys
+  // times the stride, which must hold a whole row
+  if (a->kv_tok_stride < a->head_dim || a->kv_tok_stride * 2 * kSub > 0x7fffffff)
+    return fail(PKV_ERR_UNSUPPORTED, "block_attn: kv token stride %lld (%d to %d)",
+                static_cast<long long>(a->kv_tok_stride), a->head_dim, 0x7fffffff / 2 / kSub);
   const int64_t need = pkv_block_attn_workspace_size(a);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(PKV_ERR_CAPACITY, "block_attn: workspace of %lld bytes, %lld needed",

@@ -113,6 +113,7 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, q, k, positions, freqs, axes, interleaved, scale, inverse):
         ctx.save_for_backward(positions, freqs)
         ctx.args = (axes, interleaved, scale, inverse)
+        ctx.set_materialize_grads(False)
         out = _ops.ops().rotary(q, k, positions, freqs, axes, interleaved, scale, inverse)
         return out[0] if k is None else tuple(out)
 

@@ -63,8 +63,8 @@ def _refused(rc):
 
 @pytest.mark.parametrize("fault", TILE_FAULTS + [
     dict(k=None), dict(v=None), dict(o=None), dict(kv_tok_stride=129), dict(kv_head_stride=4), dict(o_tok_stride=2),
-    dict(kv_tok_stride=-128), dict(kv_tok_stride=1 << 24), dict(softmax_scale=0.0), dict(softmax_scale=-1.0),
-    dict(softmax_scale=float("nan")), dict(softmax_scale=float("inf")), dict(max_seqlen_q=1 << 30, block_q=1),
+    dict(kv_tok_stride=-128), dict(kv_tok_stride=0), dict(kv_tok_stride=120), dict(kv_tok_stride=1 << 24), dict(softmax_scale=0.0), dict(softmax_scale=-1.0),
+    dict(softmax_scale=float("nan")), dict(softmax_scale=float("inf")), dict(max_seqlen_q=1 << 30, block_q=1), dict(max_seqlen_q=1 << 23, block_q=1),
 ], ids=str)
 def test_attention_refusals(fault):
     a = _attn(**fault)
@@ -74,7 +74,7 @@ def test_attention_refusals(fault):
 @pytest.mark.parametrize("fault", TILE_FAULTS + [
     dict(means=None), dict(sink_blocks=-1), dict(recent_blocks=-1), dict(sink_blocks=3, recent_blocks=2),
     dict(sink_blocks=0x7fffffff, recent_blocks=0x7fffffff), dict(max_seqlen_k=-1), dict(max_seqlen_k=32769 * 64),
-    dict(num_batches=65536),
+    dict(num_batches=65536), dict(num_heads_q=65536, num_heads_kv=65536),
 ], ids=str)
 def test_selection_refusals(fault):
     a = _select(**fault)
@@ -101,7 +101,7 @@ def test_attention_needs_its_workspace():
 @pytest.mark.parametrize("fault", [dict(head_dim=32), dict(block_k=100), dict(dtype=2), dict(num_heads=0),
                                    dict(num_seqs=-1), dict(total_k=-1), dict(last=-1), dict(max_seqlen_k=-1),
                                    dict(k=None), dict(means=None), dict(cu_seqlens_k=None), dict(kv_tok_stride=4),
-                                   dict(kv_head_stride=1), dict(num_seqs=65536)], ids=str)
+                                   dict(kv_head_stride=1), dict(num_seqs=1 << 24)], ids=str)
 def test_means_refusals(fault):
     a = _means(**fault)
     _refused(A.lib().pkv_block_means(ctypes.byref(a), None))

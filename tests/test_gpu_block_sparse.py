@@ -54,7 +54,7 @@ def _check_means(got, k, lens, block, used=None):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("lens,block,heads", [
     ([1], 64, None), ([0, 0], 64, 2), ([64, 0, 63, 1, 65], 64, None), ([130, 1, 700], 128, 3), ([1000, 333], 1024, 1),
-    ([513] * 7, 192, None)])
+    ([513] * 7, 192, None), ([3] * 70000, 64, None)])
 def test_means(lens, block, heads, D, dtype):
     k = rnd(sum(lens), D, dtype=dtype) if heads is None else rnd(sum(lens), heads, D, dtype=dtype)
     for longest in (0, max(lens), 1):  # (1: a bound too small only makes the launch loop)
@@ -371,6 +371,13 @@ def test_attend_neighbours_blocks(poison):
     hit[seen(1, 599), G:] = True
     assert hit.any() and torch.equal(~torch.isfinite(out), hit)
     assert torch.equal(out[~hit], want[~hit])
+    bad = k.clone()  # (a key that is no number takes its rows' sums with it)
+    bad[130, 0] = poison
+    out, lse2 = bs.block_sparse_attention(q, bad, v, cu([n]), cu([n]), n, lists, block_q=1, causal=True, return_lse=True)
+    hit[:, :G] = seen(0, 130)[:, None, None]
+    hit[:, G:] = False
+    assert torch.equal(out[~hit], want[~hit]) and torch.equal(lse2[:, ~seen(0, 130)], lse[:, ~seen(0, 130)])
+    assert torch.isnan(out[hit]).all()
 
 
 @pytest.mark.parametrize("bq", [1, 64, 200])
@@ -621,6 +628,7 @@ BREAKS = {
 }
 ATTEND_BREAKS = {
     "k of another type": lambda a: a.update(k=a["k"].half()),
+    "one key for all tokens": lambda a: a.update(k=rnd(1, 2, 64).expand(200, 2, 64), v=rnd(1, 2, 64).expand(200, 2, 64)),
     "v of other strides": lambda a: a.update(v=rnd(200, 4, 64)[:, ::2]),
     "k off 16 bytes": lambda a: a.update(k=rnd(200, 2, 72)[..., 1:65], v=rnd(200, 2, 72)[..., 1:65]),
     "flat keys of other batches": lambda a: a.update(k=rnd(200, 64), v=rnd(200, 64), cq=cu([5, 5]),

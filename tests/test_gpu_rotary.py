@@ -83,6 +83,18 @@ def test_rotary_strides(offset):
         _check(rope.rotary(q, pos, f, interleaved=interleaved, scale=s), q, pos, f, (32,), interleaved, s, False)
 
 
+def test_rotary_of_more_rows_than_a_launch_has_workgroups():
+    """256 pairs are a workgroup a row: more rows than 2^32 threads hold."""
+    rows = 0xffffffff // 256 + 3
+    q = torch.zeros(rows, 1, 512, device=DEV, dtype=BF)
+    at = torch.tensor([0, 1, rows - 4, rows - 3, rows - 2, rows - 1], device=DEV)
+    q[at] = torch.randn(6, 1, 512, device=DEV).to(BF)
+    pos = torch.arange(rows, device=DEV)
+    f = rope.rotary_frequencies(512, device=DEV)[0]
+    got = rope.rotary(q, pos, f)
+    _check(got[at], q[at], pos[at], f, (256,), True, 1.0, False)
+
+
 def test_rotary_of_empty_inputs():
     f = rope.rotary_frequencies(64, device=DEV)[0]
     pos = torch.zeros(0, dtype=torch.int64, device=DEV)
