@@ -696,7 +696,7 @@ constexpr float kSlack = 8.0f;
 // The first `keys` keys count (LANES: of each lane's row its own; a row of none
 // takes no part: its probabilities are 2^(0 S - inf), which is 0 unless S is no
 // number).
-template <int D, int NK, bool F16, bool LANES = false>
+template <int D, int NK, bool F16, bool LANES, bool FINE>
 __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (&qf)[D / 16], int keys, float c,
                                    RowState<D> &st) {
   constexpr int ROW = 2 * D;
@@ -742,18 +742,21 @@ __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (
     st.m = m;
   }
   // P is rounded to the inputs' 16-bit type for the matrix product (half a unit
-  // in the last place of each probability, as O's own rounding); the row sum
-  // takes the unrounded ones.
+  // in the last place of each probability, as O's own rounding), FINE: in two such
+  // parts, a second product that takes the rest; the row sum takes the unrounded
+  // ones.
   const float ref = none ? INFINITY : st.m == -INFINITY ? 0.0f : st.m;
   const float cl = none ? 0.0f : c;
-  typename Elem8<F16>::x8 pb[2 * NK];
+  typename Elem8<F16>::x8 pb[2 * NK], pl[FINE ? 2 * NK : 1];
 #pragma unroll
   for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][i], cl, -ref));
       st.l += e;
-      pb[2 * kb + i / 8][i % 8] = static_cast<typename Elem8<F16>::type>(e);
+      const typename Elem8<F16>::type h = static_cast<typename Elem8<F16>::type>(e);
+      pb[2 * kb + i / 8][i % 8] = h;
+      if constexpr (FINE) pl[2 * kb + i / 8][i % 8] = static_cast<typename Elem8<F16>::type>(e - static_cast<float>(h));
     }
   // V^T fragment: lane j of each 16 addresses V[k0 + j / 4][d0 + 4 (j % 4)] and
   // receives one column of the four keys
@@ -766,6 +769,8 @@ __device__ inline void attend_step(const char *kt, const char *vt, const uint4 (
       const char *p0 = vt + r0 * ROW + 16 * v_chunk<D>(r0, 4 * db + vc / 8) + 2 * (vc % 8);
       const i16x4 a8[2] = {lds_read_tr(p0), lds_read_tr(p0 + 8 * ROW)};  // (rows 8 apart lie alike)
       st.o[db] = mfma16<F16>(__builtin_bit_cast(uint4, a8), __builtin_bit_cast(uint4, pb[ks]), st.o[db]);
+      if constexpr (FINE)
+        st.o[db] = mfma16<F16>(__builtin_bit_cast(uint4, a8), __builtin_bit_cast(uint4, pl[ks]), st.o[db]);
     }
 }
 
@@ -921,7 +926,7 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
     asm volatile("" ::: "memory");
     if (e < n) copies.issue(p, blk * p.bk + off, buf ^ 1, t.tk.limit);
     const char *kt = smem + buf * 2 * TILE;
-    attend_step<D, 2, F16>(kt, kt + TILE, qf, max(0, t.tk.limit - key), p.scale_log2, st);
+    attend_step<D, 2, F16, false, false>(kt, kt + TILE, qf, max(0, t.tk.limit - key), p.scale_log2, st);
     buf ^= 1;
   }
   store_rows<D, F16>(p, t, r, st, both_sum(st.l), n > 0);
@@ -1035,7 +1040,7 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnPa
           const char *kt = smem + buf * 2 * TILE;
           const int keys = (who >> my_tile) & 1 ? max(0, my_limit - key) : 0;
           seen = seen || keys > 0;
-          attend_step<D, 2, F16, true>(kt, kt + TILE, qf, keys, p.scale_log2, st);
+          attend_step<D, 2, F16, true, false>(kt, kt + TILE, qf, keys, p.scale_log2, st);
         }
         buf ^= 1;
       }
@@ -1151,7 +1156,7 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
     }
     asm volatile("" ::: "memory");
     const char *kt = ring + buf * 2 * TILE;
-    attend_step<D, 1, F16>(kt, kt + TILE, qf, max(0, t.tk.limit - now), p.scale_log2, st);
+    attend_step<D, 1, F16, false, true>(kt, kt + TILE, qf, max(0, t.tk.limit - now), p.scale_log2, st);
   }
   const float l = both_sum(st.l);
 
