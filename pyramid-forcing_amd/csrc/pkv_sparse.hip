@@ -686,6 +686,17 @@ struct RowState {
   }
 };
 
+// whether the sum and all of O are numbers
+template <int D>
+__device__ inline bool finite(const RowState<D> &st) {
+  float check = st.l;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) check = fmaf(st.o[db][i], 0.0f, check);
+  return check - check == 0.0f;
+}
+
 // How far (log2) a row's scores may rise above its reference before O is
 // rescaled: probabilities stay below 2^8, and the rescale, which most tiles
 // do not need, is rare.
@@ -1049,12 +1060,7 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnPa
       store_rows<D, F16>(p, t, my_tile == only ? r : t.rows, st, both_sum(st.l), seen);
       continue;
     }
-    float check = st.l;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) check = fmaf(st.o[db][i], 0.0f, check);
-    const bool odd = __builtin_amdgcn_ballot_w64(r < t.rows && !(check - check == 0.0f)) != 0;
+    const bool odd = __builtin_amdgcn_ballot_w64(r < t.rows && !finite(st)) != 0;
     if (!__syncthreads_or(odd)) {
       store_rows<D, F16>(p, t, r, st, both_sum(st.l), seen);
       return;
@@ -1135,28 +1141,39 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
   // offset in its block
   const int stride = 32 * kSmallWaves * p.splits, blocks_on = stride / p.bk, keys_on = stride - blocks_on * p.bk;
   const int start = 32 * (wave * p.splits + split);
-  int e = start / p.bk, off = start - e * p.bk;
-  int key = e < n ? block(e) * p.bk + off : 0;
-  if (e < n) issue(key, 0);
-  for (int buf = 0; e < n; buf ^= 1) {
-    const int now = key;
-    e += blocks_on;
-    off += keys_on;
-    if (off >= p.bk) {
-      off -= p.bk;
-      ++e;
+  auto walk = [&](auto fine) {
+    int e = start / p.bk, off = start - e * p.bk;
+    int key = e < n ? block(e) * p.bk + off : 0;
+    wait_reads();  // (of the walk before)
+    if (e < n) issue(key, 0);
+    for (int buf = 0; e < n; buf ^= 1) {
+      const int now = key;
+      e += blocks_on;
+      off += keys_on;
+      if (off >= p.bk) {
+        off -= p.bk;
+        ++e;
+      }
+      wait_reads();  // the other buffer has been read
+      if (e < n) {
+        key = block(e) * p.bk + off;
+        issue(key, buf ^ 1);
+        wait_copies<2 * COPIES>();
+      } else {
+        wait_copies<0>();
+      }
+      asm volatile("" ::: "memory");
+      const char *kt = ring + buf * 2 * TILE;
+      attend_step<D, 1, F16, false, decltype(fine)::value>(kt, kt + TILE, qf, max(0, t.tk.limit - now), p.scale_log2, st);
     }
-    wait_reads();  // the other buffer has been read
-    if (e < n) {
-      key = block(e) * p.bk + off;
-      issue(key, buf ^ 1);
-      wait_copies<2 * COPIES>();
-    } else {
-      wait_copies<0>();
-    }
-    asm volatile("" ::: "memory");
-    const char *kt = ring + buf * 2 * TILE;
-    attend_step<D, 1, F16, false, true>(kt, kt + TILE, qf, max(0, t.tk.limit - now), p.scale_log2, st);
+  };
+  walk(std::true_type());
+  // an infinity in V is one of O, but the second part of P may be 0 or negative
+  // there, and the two parts' products NaN: such a wave takes its keys again, P in
+  // one part
+  if (__builtin_amdgcn_ballot_w64(!finite(st)) != 0) {
+    st.reset();
+    walk(std::false_type());
   }
   const float l = both_sum(st.l);
 
@@ -1287,8 +1304,9 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(BlockAttnParams p)
 // 32 bits
 constexpr int64_t kMaxThreads = 0xffffffffll;
 
-// cu_seqlens are 32-bit: rows past them belong to no sequence
-static int row_count(int64_t n) { return n < 0x7fffffff ? static_cast<int>(n) : 0x7fffffff; }
+// rows of q or k at most: cu_seqlens are 32-bit, and lengths are rounded up to
+// whole tiles and blocks (32 * 128 rows, 1,024 keys) in 32 bits
+constexpr int64_t kMaxTokens = 0x7fffffff - 4096;
 
 static bool is_16bit(int dtype) { return dtype == PKV_DTYPE_BF16 || dtype == PKV_DTYPE_FP16; }
 
@@ -1319,6 +1337,7 @@ extern "C" int pkv_block_means(const pkv_block_means_args *a, pkv_stream_t strea
   if (!a) return fail(PKV_ERR_INVALID, "block_means: NULL argument");
   if (a->num_seqs < 0 || a->num_heads <= 0 || a->total_k < 0 || a->last < 0 || a->max_seqlen_k < 0)
     return fail(PKV_ERR_INVALID, "block_means: bad sizes");
+  if (a->total_k > kMaxTokens) return fail(PKV_ERR_UNSUPPORTED, "block_means: too many rows");
   if (const int rc = check_block(a->head_dim, a->block_k, a->dtype, "block_means")) return rc;
   if (a->num_seqs == 0) return PKV_OK;
   if (!a->means || !a->cu_seqlens_k || (!a->k && a->total_k > 0))
@@ -1331,7 +1350,7 @@ extern "C" int pkv_block_means(const pkv_block_means_args *a, pkv_stream_t strea
   p.total_rows = a->total_k / a->block_k + a->num_seqs;
   p.tok = a->kv_tok_stride; p.head = a->kv_head_stride;
   p.S = a->num_seqs; p.H = a->num_heads; p.bk = a->block_k; p.last = a->last;
-  p.total_k = row_count(a->total_k);
+  p.total_k = static_cast<int>(a->total_k);
   // a wave per block and head of a sequence of the bound's length, as long as
   // those make no more workgroups than fill the chip many times (the others loop)
   const int64_t longest = a->max_seqlen_k > 0 ? a->max_seqlen_k : a->total_k;
@@ -1387,7 +1406,8 @@ static int check_select(const pkv_block_select_args *a) {
     return fail(PKV_ERR_UNSUPPORTED, "block_select: more than %d blocks", kMaxSelectBlocks);
   if (a->num_batches > 65535 || a->num_heads_kv > 65535)
     return fail(PKV_ERR_UNSUPPORTED, "block_select: more than 65535 batches or KV heads");
-  if (a->total_q > 0x7fffffff) return fail(PKV_ERR_UNSUPPORTED, "block_select: too many query rows");
+  if (a->total_q > kMaxTokens || a->max_seqlen_q > kMaxTokens || a->total_k > kMaxTokens)
+    return fail(PKV_ERR_UNSUPPORTED, "block_select: too many rows");
   return PKV_OK;
 }
 
@@ -1486,7 +1506,7 @@ extern "C" int pkv_block_select(const pkv_block_select_args *a, void *workspace,
   p.cu_q = a->cu_seqlens_q; p.cu_k = a->cu_seqlens_k; p.used = a->seqlens_k;
   p.tile_rows = a->total_q / a->block_q + a->num_batches;
   p.mean_rows = a->total_k / a->block_k + (a->kv_per_head ? heads : a->num_batches);
-  p.total_q = row_count(a->total_q); p.total_k = row_count(a->total_k);
+  p.total_q = static_cast<int>(a->total_q); p.total_k = static_cast<int>(a->total_k);
   p.q_tok = a->q_tok_stride; p.q_head = a->q_head_stride;
   p.B = a->num_batches; p.Hq = a->num_heads_q; p.Hkv = a->num_heads_kv;
   p.G = a->num_heads_q / a->num_heads_kv;
@@ -1516,7 +1536,9 @@ static int check_attn(const pkv_block_attn_args *a) {
     return fail(PKV_ERR_INVALID, "block_attn: softmax_scale must be above 0 and finite");
   const int64_t items = static_cast<int64_t>(a->num_batches) * a->num_heads_kv *
                         ((static_cast<int64_t>(a->max_seqlen_q) + a->block_q - 1) / a->block_q);
-  if (items > kMaxThreads / 512 || a->total_q > 0x7fffffff) return fail(PKV_ERR_UNSUPPORTED, "block_attn: grid too large");
+  if (a->total_q > kMaxTokens || a->max_seqlen_q > kMaxTokens || a->total_k > kMaxTokens)
+    return fail(PKV_ERR_UNSUPPORTED, "block_attn: too many rows");
+  if (items > kMaxThreads / 512) return fail(PKV_ERR_UNSUPPORTED, "block_attn: grid too large");
   return PKV_OK;
 }
 
@@ -1608,8 +1630,8 @@ extern "C" int pkv_block_attn(const pkv_block_attn_args *a, void *workspace, int
   BlockAttnParams p{};
   p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.lse = a->lse; p.lists = a->lists;
   p.cu_q = a->cu_seqlens_q; p.cu_k = a->cu_seqlens_k; p.used = a->seqlens_k;
-  p.total_q = row_count(a->total_q);
-  p.total_k = row_count(a->total_k);
+  p.total_q = static_cast<int>(a->total_q);
+  p.total_k = static_cast<int>(a->total_k);
   p.q_tok = a->q_tok_stride; p.q_head = a->q_head_stride;
   p.kv_tok = a->kv_tok_stride; p.kv_head = a->kv_head_stride;
   p.o_tok = a->o_tok_stride; p.o_head = a->o_head_stride;

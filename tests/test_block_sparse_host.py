@@ -90,6 +90,16 @@ def test_selection_needs_its_workspace():
     assert A.lib().pkv_block_select_workspace_size(ctypes.byref(_select(head_dim=96))) == 0
 
 
+@pytest.mark.parametrize("fault", [dict(total_q=(1 << 31) - 4095), dict(total_k=(1 << 31) - 4095), dict(total_k=1 << 31),
+                                   dict(max_seqlen_q=(1 << 31) - 4095)], ids=str)
+def test_sizes_that_rounding_up_would_wrap(fault):
+    """Lengths are rounded up to whole tiles and blocks in 32 bits."""
+    _refused(A.lib().pkv_block_attn(ctypes.byref(_attn(**dict(dict(block_q=128, num_heads_q=1), **fault))), FAKE, 1 << 40, None))
+    _refused(A.lib().pkv_block_select(ctypes.byref(_select(**fault)), FAKE, 1 << 40, None))
+    if "total_k" in fault:
+        _refused(A.lib().pkv_block_means(ctypes.byref(_means(**fault)), None))
+
+
 def test_attention_needs_its_workspace():
     a = _attn(block_q=1, max_seqlen_q=1, topk=64)  # one token over 4,096 keys: split over workgroups
     need = A.lib().pkv_block_attn_workspace_size(ctypes.byref(a))

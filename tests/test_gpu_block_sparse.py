@@ -428,6 +428,23 @@ def test_attend_infinities(bq):
     assert torch.isnan(out).all() and (lse == -INF).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("tokens,bq,topk", [(1, 1, 5), (1, 1, 18), (300, 1, 5), (40, 40, 5)])
+def test_attend_infinite_values(tokens, bq, topk, dtype):
+    """An infinity among the listed values is one of its column, two of opposite
+    signs NaN, and the other columns are as without it."""
+    n = 64 * topk - 20
+    q, k, v = rnd(tokens, 2, 64, dtype=dtype), rnd(n, 64, dtype=dtype), rnd(n, 64, dtype=dtype)
+    v[:, :3] = 0
+    lists = torch.arange(topk, dtype=torch.int32, device=DEV).expand(tokens // bq + 1, 1, topk).contiguous()
+    vv = v.clone()
+    vv[7, 0], vv[70, 1], vv[n - 1, 2], vv[n - 3, 2] = INF, -INF, INF, -INF
+    out, lse = bs.block_sparse_attention(q, k, vv, cu([tokens]), cu([n]), tokens, lists, block_q=bq, return_lse=True)
+    assert (out[..., 0] == INF).all() and (out[..., 1] == -INF).all() and torch.isnan(out[..., 2]).all()
+    out[..., :3] = 0
+    _attend_check(out, lse, q, k, v, lists, [tokens], [n], 1, True, bq, 64)
+
+
 def test_attend_strides_rows_in_use_and_other_rows():
     """q, k and v as slices of wider buffers, keys in use, an output whose other rows stay."""
     q_lens, k_lens, used = [30, 5], [300, 260], [129, 260]
