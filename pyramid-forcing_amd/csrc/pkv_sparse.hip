@@ -59,8 +59,13 @@ __device__ inline Span key_span(const int32_t *cu, const int32_t *used, int s, i
 
 // ---- block means -----------------------------------------------------------
 // One wave per block and head: lane i takes 8 columns of every 64 / (D / 8)-th
-// key in 16-byte reads, all in flight together, then the lanes of a column are
-// added.  Sums in fp32, 16 keys a lane before the lanes are joined.
+// key in 16-byte reads, 64 keys in flight together, then the lanes of a column
+// are added.  Sums in fp32: a lane's keys in turn (16 of a block of 64 at head_dim
+// 128), then the lanes' in a tree.
+// Bound by memory, every key read once: 36 sequences of 6,240 to 32,760 keys
+// (188 MB) in 34.7 us, 5.4 TB/s (a copy of 1 GiB moves 4.8); 3 sequences of 300
+// keys in 4.2, most of it the launch.  Workgroups of a sequence lie together: with
+// the sequences fastest the same call took 38.8.
 struct MeansParams {
   const uint16_t *k;
   float *means;
@@ -123,9 +128,10 @@ __global__ void __launch_bounds__(256) block_means_kernel(MeansParams p) {
 }
 
 // ---- block selection ---------------------------------------------------------
-// Scores and choice in two launches: a tile's scores go through the workspace
-// as ordered 32-bit keys (larger score, larger key), so that the launch that
-// reads the means splits over blocks and tiles as it likes.
+// Scores and choice in two launches, or three with the tiles' sums: a tile's
+// scores go through the workspace as ordered 32-bit keys (larger score, larger
+// key), so that the launch that reads the means splits over blocks and tiles as
+// it likes; or all in one launch (block_select_kernel).
 //
 // The score's sums are taken in fp64: the choice is then the one of the formula
 // (two blocks change places only where their scores agree to 1e-15), whatever
@@ -218,7 +224,8 @@ __device__ inline double add_lane32(double x) {
          __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
 }
 
-// the tile's summed query rows: grid (tiles, Hkv, B)
+// The tile's summed query rows: grid (tiles, Hkv, B).  468 tiles of 120 rows of
+// head_dim 128 (14.4 MB) in 5.3 us: the launch, two dependent reads and the tree.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) tile_sums_kernel(SelectParams p) {
   constexpr int LPR = D / 8, ROWS = 256 / LPR;
@@ -252,6 +259,9 @@ __device__ inline uint32_t score_key(float f) {
 // so that the 4 lanes of a block read 64 bytes together (a lane's quarter of the
 // row in one piece had every read touch 64 cache lines, and again for each of
 // its 8 parts); result: lane l holds block l % 16 of tiles l / 16 + 4 i.
+// 36 groups of 13 tiles and 98 to 512 blocks each in 8.2 us: a chain of dependent
+// reads (lengths, sums, means) and 32 matrix instructions.  Four chains of those
+// and the means read before the sums: 8.6.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) block_scores_kernel(SelectParams p) {
   constexpr int C = D / 4;  // columns of a lane
@@ -316,9 +326,9 @@ __global__ void __launch_bounds__(256) block_scores_kernel(SelectParams p) {
 // Writes the want = min(topk, n) largest of a row's keys, ascending by index and
 // padded with -1, to out.  W waves of R keys a lane take part: wave w holds keys
 // [w * 64 * R, ...), lane l of it keys l, l + 64, ...; 0 where there is none.
-// The want-th largest is found bit by bit, counting with ballots; ties at it go
-// to the lowest indices.  counts: 2 * W ints of LDS (W > 1, where the whole
-// workgroup calls it).
+// The want-th largest is found bit by bit, counting with ballots (at most 32 rounds
+// over keys in registers, whatever topk is); ties at it go to the lowest indices.
+// counts: 2 * W ints of LDS (W > 1, where the whole workgroup calls it).
 template <int W, int R>
 __device__ inline void choose(const uint32_t (&key)[R], int n, int topk, int32_t *out, int *counts) {
   const int lane = threadIdx.x & 63, wave = W > 1 ? threadIdx.x >> 6 : 0;
@@ -397,7 +407,8 @@ __device__ inline void clear_rows(const SelectParams &p, int b, int h, int64_t f
 
 // A row (tile, KV head) of the lists from block_scores_kernel's keys: one per
 // workgroup of W waves, or, W 1, one per wave and 4 per workgroup.  Grid: (tiles,
-// Hkv, B).
+// Hkv, B).  468 rows of 98 to 512 keys in 5.3 us, most of it the launch and the
+// rounds of the search.
 template <int W, int R>
 __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(SelectParams p) {
   __shared__ int counts[2 * W];
@@ -432,7 +443,10 @@ __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(Sele
 // (W 1: 4 rows a workgroup, each wave by itself), grid (tiles, Hkv, B).  The row's summed queries and
 // its keys lie in LDS; 4 lanes take a block's mean, 16 blocks a wave at a time,
 // in vector fp64.  A row of the lists costs nb * 4 D bytes of means, which the
-// rows of a sequence do not share as block_scores_kernel's 16 do.
+// rows of a sequence do not share as block_scores_kernel's 16 do: bound by what a
+// compute unit reads (16 tokens of 8 KV heads, 63 to 512 blocks, in 12.5 us: the
+// longest row's 262 KB at about 20 bytes a clock, and the search; 2,047 tokens of 2
+// KV heads, up to 32 blocks, in 11.8).
 template <int D, bool F16, int W, int R>
 __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_select_kernel(SelectParams p) {
   constexpr int ROWS = W > 1 ? 1 : 4, NB = W * 64 * R;  // rows of a workgroup, keys of a row
@@ -900,7 +914,19 @@ struct TileCopies {
 };
 
 // Tiles of up to 32 W rows: W waves of 32 rows, the keys in steps of 64 through
-// two LDS buffers that all waves share.
+// two LDS buffers that all waves share; two workgroups on a compute unit, so that
+// one's matrix instructions run beside the other's exponentials.
+//
+// 468 tiles of 120 rows over 6,400 keys each (bf16, head_dim 128; 184 GFLOP) take
+// 220 to 237 us, 775 to 835 TFLOP/s, where a large library product reaches 1,200 on
+// the same card.  Matrix units are busy 56% of the time of the units that have
+// work; without the copies it takes 178 us, without LDS reads too 145, without
+// exponentials too 121: copies, fragment reads and exponentials each take time
+// that the matrix instructions of two waves a SIMD do not cover, and every tile has
+// a list of its own, so that no other rows could share its copies.  Not faster:
+// steps of 32 keys in a ring of four; the scores of the next step beside the
+// exponentials of this one (219 to 240 in all orders tried); 64 rows a wave (260);
+// raised wave priority; touching the next blocks ahead (235 to 268).
 template <int D, int W, bool F16>
 __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnParams p) {
   constexpr int ROW = 2 * D, TILE = kSub * ROW;  // bytes
@@ -953,6 +979,11 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
 // blocks that only its neighbours list: where that is not 0 (V holds an
 // infinity or NaN) the results say so, and the workgroup takes its tiles one by
 // one instead.
+//
+// 2,047 tokens of 2 KV heads and 16 query heads each, 16 blocks a token (fp16,
+// head_dim 128) in 55 to 57 us; the small kernel, one token a workgroup, 208.
+// Bound by its longest workgroup: 128 of them, a step's copies, reads and
+// exponentials one after the other as in the tile kernel.
 constexpr int kWindow = 1024;    // blocks whose lists are joined at a time
 constexpr int kMaxGroup = 32;    // tiles: a bit each
 constexpr int kGroupItems = 128; // workgroups that a launch in groups has at least
@@ -1072,6 +1103,10 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnPa
 // take every fourth 32-key step of the list through a ring of their own, with
 // no barrier in the loop, joined at the end.  splits > 1 divides the list over
 // as many workgroups, whose parts block_attn_join_kernel adds up.
+//
+// Bound by memory: 16 tokens of 8 KV heads over 32 blocks each (134 MB of K and V)
+// take 25 us here, 5.3 TB/s, and 4 in the join; one token of 2 KV heads over 8 blocks
+// 7.2, a chain of dependent reads (lengths, list, keys) and the launch.
 constexpr int kSmallWaves = 4;
 constexpr int kRing = 2;
 
