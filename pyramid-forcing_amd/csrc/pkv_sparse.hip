@@ -557,6 +557,7 @@ struct BlockAttnParams {
   int B, Hq, Hkv, G, per_head;
   int tiles, items;  // tiles (groups of tiles) of the longest sequence; B * Hkv * tiles
   int group;         // tiles that a workgroup takes together
+  int max_q;         // tokens of the longest sequence: later ones are left alone
   int bq, bk, topk, causal;
   float scale_log2;
   int splits;        // workgroups of an item
@@ -821,8 +822,9 @@ __device__ inline bool attn_tile(const BlockAttnParams &p, int item, AttnTile &t
   t.q_begin = q.begin;
   t.Lq = q.n;
   t.tok0 = tile * p.group * p.bq;
-  if (t.tok0 >= t.Lq) return false;
-  const int tokens = min(p.group * p.bq, t.Lq - t.tok0);
+  const int left = min(t.Lq, p.max_q) - t.tok0;
+  if (left <= 0) return false;
+  const int tokens = min(p.group * p.bq, left);
   t.rows = tokens * p.G;
   t.tk = tile_keys(p, t.b, t.h, t.Lq, (t.tok0 + tokens - 1) / p.bq);
   return true;
@@ -1677,6 +1679,7 @@ extern "C" int pkv_block_attn(const pkv_block_attn_args *a, void *workspace, int
   p.tiles = static_cast<int>(s.tiles);
   p.items = static_cast<int>(s.items);
   p.group = s.group;
+  p.max_q = a->max_seqlen_q;
   p.bq = a->block_q; p.bk = a->block_k; p.topk = a->topk;
   p.causal = a->causal ? 1 : 0;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;

@@ -477,6 +477,28 @@ def test_attend_strides_rows_in_use_and_other_rows():
         _attend_check(o[:35], lse[:, :35], q[:35], kc, vc, lists, q_lens, k_lens, 2, False, bq, 64, used=used)
 
 
+@pytest.mark.parametrize("q_len,most,bq", [(30, 17, 4), (300, 257, 1), (90, 50, 30), (5, 5, 1), (5, 9, 8)])
+def test_attend_leaves_tokens_past_the_longest(q_len, most, bq):
+    """Tokens past max_seqlen_q stay as they were, where they share a tile or a
+    workgroup with earlier ones too."""
+    q, k, v = rnd(q_len, 4, 64), rnd(300, 2, 64), rnd(300, 2, 64)
+    lists = _lists([q_len], [300], 2, False, bq, 64, 5, np.random.default_rng(5))
+    o, lse = torch.full((q_len, 4, 64), 3.0, dtype=BF, device=DEV), torch.full((4, q_len), 3.0, device=DEV)
+    cq, ck = cu([q_len]), cu([300])
+    a = A.BlockAttnArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), lse=lse.data_ptr(),
+                        lists=lists.data_ptr(), cu_seqlens_q=cq.data_ptr(), cu_seqlens_k=ck.data_ptr(), total_q=q_len,
+                        total_k=300, q_tok_stride=256, q_head_stride=64, kv_tok_stride=128, kv_head_stride=64,
+                        o_tok_stride=256, o_head_stride=64, num_batches=1, num_heads_q=4, num_heads_kv=2, head_dim=64,
+                        max_seqlen_q=most, block_q=bq, block_k=64, topk=5, softmax_scale=0.125)
+    need = A.lib().pkv_block_attn_workspace_size(ctypes.byref(a))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    A.check(A.lib().pkv_block_attn(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), need, stream), "block_attn")
+    assert (o[most:] == 3.0).all() and (lse[:, most:] == 3.0).all()
+    n = min(most, q_len)
+    _attend_check(o[:n], lse[:, :n], q[:n], k, v, lists, [n], [300], 2, False, bq, 64)
+
+
 def test_attend_past_32_bit_offsets():
     rows = 66000
     buf = torch.empty(rows, 1 << 16, dtype=BF, device=DEV)
