@@ -142,7 +142,9 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, k: 
     all by one).  freqs: float64, one a pair (rotary_frequencies); angles are
     taken in 64 bits, so positions may be far.  Pair j is columns 2j and 2j + 1
     (interleaved) or j and j + pairs; columns from twice the pairs on are
-    copied.  inverse turns back.  Differentiable in q and k."""
+    copied.  inverse turns back.  Differentiable in q and k; a graph that captures
+    the backward pass too needs leaves that no living eager result was computed
+    from (torch ends the process otherwise)."""
     axes = (int(freqs.numel()),) if axes is None else tuple(int(a) for a in axes)
     args = (positions, freqs, axes, bool(interleaved), float(scale), bool(inverse))
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):

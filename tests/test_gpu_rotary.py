@@ -201,6 +201,37 @@ def test_rotary_replayed():
         assert torch.equal(out, rope.rotary(q, pos, f))
 
 
+def test_rotary_gradient_replayed():
+    """Forward and backward in one graph, of leaves that no eager result uses."""
+    f, pos = rope.rotary_frequencies(64, device=DEV)[0], torch.randint(0, 9999, (40,), device=DEV)
+
+    def step(q, k, g):
+        out = rope.rotary(q, pos, f, k=k, interleaved=False)
+        return torch.autograd.grad(out, (q, k), g)
+
+    def leaves():
+        return [torch.randn(40, h, 64, device=DEV).to(BF).requires_grad_() for h in (4, 2)]
+
+    g = [torch.randn(40, h, 64, device=DEV).to(BF) for h in (4, 2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves(), g)
+    torch.cuda.synchronize()
+    q, k = leaves()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dq, dk = step(q, k, g)
+    for i in range(4):
+        for x in g:
+            x.copy_(torch.randn_like(x))
+        pos.copy_(torch.randint(0, 9999, (40,), device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        eq, ek = step(*leaves(), g)
+        assert torch.equal(dq, eq) and torch.equal(dk, ek)
+
+
 Z = lambda *s, dtype=BF, device=DEV: torch.zeros(s, dtype=dtype, device=device)
 REFUSED = {
     "q of two dimensions": lambda: dict(q=Z(4, 64)),
