@@ -991,7 +991,7 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
 // the other as in the tile kernel.
 constexpr int kWindow = 1024;    // blocks whose lists are joined at a time
 constexpr int kMaxGroup = 32;    // tiles: a bit each
-constexpr int kGroupItems = 128; // workgroups that a launch in groups has at least
+constexpr int kGroupItems = 512; // workgroups that the chip takes in one round, two a unit
 
 template <int D, int W, bool F16>
 __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnParams p) {
@@ -1600,12 +1600,15 @@ static AttnPlan attn_plan(const pkv_block_attn_args *a) {
   const int64_t tiles = (static_cast<int64_t>(a->max_seqlen_q) + a->block_q - 1) / a->block_q;
   s.group = s.splits = 1;
   if (rows <= 32) {
-    // as many tiles as make 128 rows, fewer where that leaves compute units
-    // without a workgroup
-    int64_t g = 128 / rows < kMaxGroup ? 128 / rows : kMaxGroup;
-    if (g > tiles) g = tiles;
-    while (g > 1 && heads * ((tiles + g - 1) / g) < kGroupItems) g /= 2;
-    if (g > 1) s.group = static_cast<int>(g);
+    // as few tiles a workgroup as the chip takes in one round, up to 128 rows.  Tokens of
+    // 2 KV heads of 16 query heads, 16 blocks each of the same 512 / of lists of their
+    // own: 256 tokens one by one 33 / 36 us, by fours 47 / 98; 512 by twos 42 / 58, one
+    // by one 59 / 67, by eights 41 / 134; 1,500 by eights 60 / 152, by fours (two
+    // rounds) 95 / 190, one by one 163 / 181
+    const int64_t most = 128 / rows < kMaxGroup ? 128 / rows : kMaxGroup;
+    int64_t g = 1;
+    while (g < most && heads * ((tiles + g - 1) / g) > kGroupItems) g = 2 * g < most ? 2 * g : most;
+    s.group = static_cast<int>(g);
   }
   s.tiles = (tiles + s.group - 1) / s.group;
   s.items = heads * s.tiles;

@@ -351,6 +351,17 @@ def test_attend(case, D, dtype):
         assert torch.equal(out, again)
 
 
+def test_attend_in_the_largest_groups():
+    """32 tiles of 2 rows to a workgroup, more than one window of blocks long."""
+    q_len, k_len, hkv = 1400, 66000, 6
+    q, k, v = rnd(q_len, 2 * hkv, 64), rnd(k_len, hkv, 64), rnd(k_len, hkv, 64)
+    lists = _lists([q_len], [k_len], hkv, False, 1, 64, 3, np.random.default_rng(8))
+    out, lse = bs.block_sparse_attention(q, k, v, cu([q_len]), cu([k_len]), q_len, lists, block_q=1, return_lse=True)
+    assert torch.isfinite(out).all()
+    some = torch.arange(0, q_len, 7, device=DEV)  # (every seventh token, as a sequence of its own lists)
+    _attend_check(out[some], lse[:, some], q[some], k, v, lists[:q_len][some], [len(some)], [k_len], hkv, False, 1, 64)
+
+
 @pytest.mark.parametrize("poison", [float("nan"), INF])
 def test_attend_neighbours_blocks(poison):
     """Tiles that a workgroup takes together: a value that is no number reaches
@@ -429,7 +440,7 @@ def test_attend_infinities(bq):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF], ids=str)
-@pytest.mark.parametrize("tokens,bq,topk", [(1, 1, 5), (1, 1, 18), (300, 1, 5), (40, 40, 5)])
+@pytest.mark.parametrize("tokens,bq,topk", [(1, 1, 5), (1, 1, 18), (300, 1, 5), (600, 1, 5), (40, 40, 5)])
 def test_attend_infinite_values(tokens, bq, topk, dtype):
     """An infinity among the listed values is one of its column, two of opposite
     signs NaN, and the other columns are as without it."""
