@@ -562,7 +562,8 @@ struct BlockAttnParams {
   int bq, bk, topk, causal;
   float scale_log2;
   int splits;        // workgroups of an item
-  float *part;       // splits > 1: [items, splits, 32, D + 4]
+  int part_rows;     // rows of a part: those of the workgroup's waves
+  float *part;       // splits > 1: [items, splits, part_rows, D + 4]
 };
 
 template <int N>
@@ -879,6 +880,13 @@ __device__ inline void store_rows(const BlockAttnParams &p, const AttnTile &t, i
   if (p.lse && hf == 0) p.lse[static_cast<int64_t>(head) * p.total_q + row] = log_sum(st.m, l);
 }
 
+// Row r of a split item's part: O, the reference, the sum, whether any key was
+// seen
+template <int D>
+__device__ inline float *part_row(const BlockAttnParams &p, int item, int split, int r) {
+  return p.part + ((static_cast<int64_t>(item) * p.splits + split) * p.part_rows + r) * (D + 4);
+}
+
 // The copies of 64 keys' K and V rows into one of two buffers, by W waves
 // together
 template <int D, int W>
@@ -919,7 +927,9 @@ struct TileCopies {
 
 // Tiles of up to 32 W rows: W waves of 32 rows, the keys in steps of 64 through
 // two LDS buffers that all waves share; two workgroups on a compute unit, so that
-// one's matrix instructions run beside the other's exponentials.
+// one's matrix instructions run beside the other's exponentials.  splits > 1
+// divides the list over as many workgroups, whose parts block_attn_join_kernel
+// adds up.
 //
 // 468 tiles of 120 rows over 6,400 keys each (bf16, head_dim 128; 184 GFLOP) take
 // 220 to 237 us, 775 to 835 TFLOP/s, where a large library product reaches 1,200 on
@@ -938,7 +948,9 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
   __shared__ int list[kMaxTopk + 2];
   __shared__ int scratch[2];
   AttnTile t;
-  if (!attn_tile(p, xcd_order(blockIdx.x, p.items), t)) return;
+  const int wg = xcd_order(blockIdx.x, p.items * p.splits);
+  const int item = wg / p.splits, split = wg - item * p.splits;
+  if (!attn_tile(p, item, t)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = __builtin_amdgcn_readfirstlane(load_list<64 * W>(tile_list(p, t), p.topk, t.tk.blocks, list, scratch));
   const int r = 32 * wave + (threadIdx.x & 31);
@@ -949,11 +961,17 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
   st.reset();
 
   const TileCopies<D, W> copies(p, t, smem, wave);
-  int blk = __builtin_amdgcn_readfirstlane(list[0]), off = 0, buf = 0;
-  int nxt = list[1];  // (past the last block it may be anything)
-  if (n > 0) copies.issue(p, blk * p.bk, 0, t.tk.limit);
-  for (int e = 0; e < n;) {
+  // this workgroup's steps of the list's, from a block and an offset in it on
+  const int per = p.bk / kSub, steps = n * per;
+  const int first = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
+  const int last = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
+  int e = first / per, off = (first - e * per) * kSub, buf = 0;
+  int blk = __builtin_amdgcn_readfirstlane(list[e]);
+  int nxt = list[e + 1];  // (past the last block it may be anything)
+  if (first < last) copies.issue(p, blk * p.bk + off, 0, t.tk.limit);
+  for (int step = first; step < last;) {
     const int key = blk * p.bk + off;
+    ++step;
     off += kSub;
     if (off == p.bk) {
       off = 0;
@@ -965,12 +983,26 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
     wait_reads();
     __builtin_amdgcn_s_barrier();  // the step has arrived, and no wave reads the other buffer any more
     asm volatile("" ::: "memory");
-    if (e < n) copies.issue(p, blk * p.bk + off, buf ^ 1, t.tk.limit);
+    if (step < last) copies.issue(p, blk * p.bk + off, buf ^ 1, t.tk.limit);
     const char *kt = smem + buf * 2 * TILE;
     attend_step<D, 2, F16, false, false>(kt, kt + TILE, qf, max(0, t.tk.limit - key), p.scale_log2, st);
     buf ^= 1;
   }
-  store_rows<D, F16>(p, t, r, st, both_sum(st.l), n > 0);
+  const float l = both_sum(st.l);
+  if (p.splits == 1) {
+    store_rows<D, F16>(p, t, r, st, l, n > 0);
+    return;
+  }
+  if (r >= t.rows) return;
+  const int hf = (threadIdx.x & 63) >> 5;
+  float *part = part_row<D>(p, item, split, r);
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<float4 *>(part + 32 * db + 8 * i + 4 * hf) =
+          make_float4(st.o[db][4 * i], st.o[db][4 * i + 1], st.o[db][4 * i + 2], st.o[db][4 * i + 3]);
+  if (hf == 0) *reinterpret_cast<float4 *>(part + D) = make_float4(st.m, l, n > 0 ? 1.0f : 0.0f, 0.0f);
 }
 
 // Several consecutive small tiles at once (a prompt in which every token has a
@@ -1115,12 +1147,6 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnPa
 constexpr int kSmallWaves = 4;
 constexpr int kRing = 2;
 
-template <int D>
-struct PartLayout {
-  static constexpr int kRow = D + 4;  // O, reference, sum, whether any key was seen
-  static constexpr int kFloats = 32 * kRow;
-};
-
 template <int D, bool F16>
 __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(BlockAttnParams p) {
   constexpr int ROW = 2 * D, TILE = 32 * ROW;
@@ -1247,7 +1273,7 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
   const int tok = lq / p.G, g = lq - tok * p.G, head = t.h * p.G + g;
   const int64_t row = t.q_begin + static_cast<int64_t>(t.tok0) + tok;
   const float inv = inv_sum(sum, n > 0);
-  float *part = p.part + (static_cast<int64_t>(item) * p.splits + split) * PartLayout<D>::kFloats + lq * PartLayout<D>::kRow;
+  float *part = part_row<D>(p, item, split, lq);
 #pragma unroll
   for (int i = wave; i < QUADS; i += kSmallWaves) {
     float4 a = buf[i * 64 + lane];
@@ -1281,7 +1307,8 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
 // columns i and i + 64; parts are read eight together.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) block_attn_join_kernel(BlockAttnParams p) {
-  constexpr int FLOATS = PartLayout<D>::kFloats, C = D / 64, kAhead = 8;
+  constexpr int C = D / 64, kAhead = 8;
+  const int64_t part_floats = static_cast<int64_t>(p.part_rows) * (D + 4);  // from part to part
   const int rows = p.bq * p.G;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int item = static_cast<int>(w / rows), r = static_cast<int>(w - static_cast<int64_t>(item) * rows);
@@ -1289,15 +1316,15 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(BlockAttnParams p)
   AttnTile t;
   if (!attn_tile(p, item, t) || r >= t.rows) return;
   const int lane = threadIdx.x & 63;
-  const float *part = p.part + static_cast<int64_t>(item) * p.splits * FLOATS + r * PartLayout<D>::kRow;
+  const float *part = part_row<D>(p, item, 0, r);
   float m = -INFINITY, sum = 0.0f, o[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] = 0.0f;
   bool keys = false;
   for (int s0 = 0; s0 < p.splits; s0 += 64) {
     const int cnt = min(64, p.splits - s0);
-    const float *x = part + static_cast<int64_t>(s0) * FLOATS;
-    const float4 mine = lane < cnt ? *reinterpret_cast<const float4 *>(x + static_cast<int64_t>(lane) * FLOATS + D)
+    const float *x = part + s0 * part_floats;
+    const float4 mine = lane < cnt ? *reinterpret_cast<const float4 *>(x + lane * part_floats + D)
                                    : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
     float top = mine.x, add;
 #pragma unroll
@@ -1319,7 +1346,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(BlockAttnParams p)
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int c = 0; c < C; ++c) v[i][c] = x[static_cast<int64_t>(min(s + i, cnt - 1)) * FLOATS + 64 * c + lane];
+        for (int c = 0; c < C; ++c) v[i][c] = x[min(s + i, cnt - 1) * part_floats + 64 * c + lane];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const float fi = __shfl(f, s + i);
@@ -1590,7 +1617,7 @@ static int check_attn(const pkv_block_attn_args *a) {
 // share a tile.
 struct AttnPlan {
   int64_t tiles, items;  // groups of a sequence, of all
-  int group, splits;
+  int group, splits, part_rows;
 };
 
 static AttnPlan attn_plan(const pkv_block_attn_args *a) {
@@ -1622,6 +1649,19 @@ static AttnPlan attn_plan(const pkv_block_attn_args *a) {
     if (n > steps) n = steps;
     if (steps >= 8 && n > 1) s.splits = static_cast<int>(n);
   }
+  s.part_rows = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  if (rows > 32 && s.items > 0) {
+    // one round of the chip (two workgroups on a unit, one of 8 waves) where it takes
+    // three a tile, each at least four steps of 64 keys: 12 tiles of 120 rows and 64
+    // blocks 24.5 us (83.7 alone; 25.3 in pieces of 8 steps, 32.8 of 16), a token of 2
+    // KV heads of 48 query heads and 15 blocks 16.3 (25.8; 26.5 in pieces of 8), 156
+    // tiles of 128 rows and 64 blocks 72 in threes (91), but 200 of 32 blocks 61 in
+    // twos (51)
+    const int64_t places = (rows <= 128 ? 512 : 256) / s.items;
+    const int64_t pieces = static_cast<int64_t>(a->topk) * (a->block_k / kSub) / 4;
+    const int64_t n = places < pieces ? places : pieces;
+    if (places >= 3 && n > 1) s.splits = static_cast<int>(n);
+  }
   return s;
 }
 
@@ -1637,11 +1677,12 @@ static int launch_block_attn(const BlockAttnParams &p, hipStream_t st) {
   if (rows > 32) {
     const int w = rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
     auto *k = w == 2 ? block_attn_tile_kernel<D, 2, F16> : w == 4 ? block_attn_tile_kernel<D, 4, F16> : block_attn_tile_kernel<D, 8, F16>;
-    hipLaunchKernelGGL(k, dim3(p.items), dim3(64 * w), 0, st, p);
-    return check_launch("block_attn_tile_kernel");
+    hipLaunchKernelGGL(k, dim3(p.items * p.splits), dim3(64 * w), 0, st, p);
+    if (const int rc = check_launch("block_attn_tile_kernel")) return rc;
+  } else {
+    hipLaunchKernelGGL((block_attn_small_kernel<D, F16>), dim3(p.items * p.splits), dim3(64 * kSmallWaves), 0, st, p);
+    if (const int rc = check_launch("block_attn_small_kernel")) return rc;
   }
-  hipLaunchKernelGGL((block_attn_small_kernel<D, F16>), dim3(p.items * p.splits), dim3(64 * kSmallWaves), 0, st, p);
-  if (const int rc = check_launch("block_attn_small_kernel")) return rc;
   if (p.splits == 1) return PKV_OK;
   const int64_t waves = static_cast<int64_t>(p.items) * rows;
   hipLaunchKernelGGL((block_attn_join_kernel<D, F16>), dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, st, p);
@@ -1653,7 +1694,7 @@ static int launch_block_attn(const BlockAttnParams &p, hipStream_t st) {
 extern "C" int64_t pkv_block_attn_workspace_size(const pkv_block_attn_args *a) {
   if (!a || check_attn(a)) return 0;
   const AttnPlan s = attn_plan(a);
-  return s.splits > 1 ? s.items * s.splits * 32 * (a->head_dim + 4) * 4 : 0;
+  return s.splits > 1 ? s.items * s.splits * s.part_rows * (a->head_dim + 4) * 4 : 0;
 }
 
 extern "C" int pkv_block_attn(const pkv_block_attn_args *a, void *workspace, int64_t workspace_bytes,
@@ -1694,6 +1735,7 @@ extern "C" int pkv_block_attn(const pkv_block_attn_args *a, void *workspace, int
   p.causal = a->causal ? 1 : 0;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.splits = s.splits;
+  p.part_rows = s.part_rows;
   p.part = static_cast<float *>(workspace);
   hipStream_t st = as_stream(stream);
   const bool f16 = a->dtype == PKV_DTYPE_FP16;

@@ -327,6 +327,10 @@ ATTEND = [  # q lens, k lens, hkv, G, per_head, topk, bq, bk, causal
     ([700], [700], 2, 8, False, 6, 1, 64, True), ([310, 250], [900, 100], 2, 16, False, 5, 1, 64, True),
     ([2047], [1500], 1, 16, False, 3, 1, 128, True), ([1000], [640], 3, 1, True, 4, 4, 64, False),
     ([1030], [70000], 1, 8, False, 8, 2, 64, False), ([5, 900], [0, 300], 1, 7, False, 2, 3, 64, False),
+    # few tiles of many rows: split over workgroups
+    ([120], [5000], 2, 1, True, 40, 120, 64, False), ([1], [9000], 1, 48, False, 80, 1, 64, False),
+    ([40, 3], [3000, 0], 1, 6, False, 24, 40, 64, False), ([70], [20000], 1, 2, False, 9, 32, 1024, False),
+    ([1, 1], [2500, 130], 1, 128, False, 33, 1, 64, True), ([9], [70000], 1, 16, False, 1024, 9, 64, False),
 ]
 
 
@@ -440,7 +444,7 @@ def test_attend_infinities(bq):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF], ids=str)
-@pytest.mark.parametrize("tokens,bq,topk", [(1, 1, 5), (1, 1, 18), (300, 1, 5), (600, 1, 5), (40, 40, 5)])
+@pytest.mark.parametrize("tokens,bq,topk", [(1, 1, 5), (1, 1, 18), (300, 1, 5), (600, 1, 5), (40, 40, 5), (40, 40, 40)])
 def test_attend_infinite_values(tokens, bq, topk, dtype):
     """An infinity among the listed values is one of its column, two of opposite
     signs NaN, and the other columns are as without it."""
