@@ -887,13 +887,13 @@ __device__ inline float *part_row(const BlockAttnParams &p, int item, int split,
   return p.part + ((static_cast<int64_t>(item) * p.splits + split) * p.part_rows + r) * (D + 4);
 }
 
-// The copies of 64 keys' K and V rows into one of two buffers, by W waves
-// together
-template <int D, int W>
+// The copies of a step's K and V rows (STEP keys) into one of two buffers, by W
+// waves together
+template <int D, int W, int STEP>
 struct TileCopies {
-  static constexpr int ROW = 2 * D, TILE = kSub * ROW;
+  static constexpr int ROW = 2 * D, TILE = STEP * ROW;
   static constexpr int RPC = 64 / (D / 8);       // rows of a copy
-  static constexpr int COPIES = kSub / RPC / W;  // a wave's copies of K, and of V
+  static constexpr int COPIES = STEP / RPC / W;  // a wave's copies of K, and of V
   const uint16_t *k, *v;
   int row_bytes;
   uint32_t lds;
@@ -912,9 +912,9 @@ struct TileCopies {
       vvoff[i] = row * row_bytes + 16 * v_chunk<D>(row, pos);
     }
   }
-  // keys [key, key + 64) below `limit`
+  // keys [key, key + STEP) below `limit`
   __device__ void issue(const BlockAttnParams &p, int key, int buf, int limit) const {
-    const int left = max(0, min(kSub, limit - key));
+    const int left = max(0, min(STEP, limit - key));
     const int64_t off = left > 0 ? key * p.kv_tok : 0;
     const uint32_t dst = lds + buf * 2 * TILE;
 #pragma unroll
@@ -927,7 +927,10 @@ struct TileCopies {
 
 // Tiles of up to 32 W rows: W waves of 32 rows, the keys in steps of 64 through
 // two LDS buffers that all waves share; two workgroups on a compute unit, so that
-// one's matrix instructions run beside the other's exponentials.  splits > 1
+// one's matrix instructions run beside the other's exponentials.  Two waves (up to
+// 64 rows) leave half of the unit's room for waves empty so, and take steps of 32
+// where there are workgroups for four on a unit: 1,024 tiles of 64 rows and 32
+// blocks 88 us (107 in steps of 64), but 400 of 48 rows 69 (55).  splits > 1
 // divides the list over as many workgroups, whose parts block_attn_join_kernel
 // adds up.
 //
@@ -941,9 +944,9 @@ struct TileCopies {
 // steps of 32 keys in a ring of four; the scores of the next step beside the
 // exponentials of this one (219 to 240 in all orders tried); 64 rows a wave (260);
 // raised wave priority; touching the next blocks ahead (235 to 268).
-template <int D, int W, bool F16>
+template <int D, int W, int STEP, bool F16>
 __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnParams p) {
-  constexpr int ROW = 2 * D, TILE = kSub * ROW;  // bytes
+  constexpr int ROW = 2 * D, TILE = STEP * ROW;  // bytes
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];  // K0 V0 K1 V1
   __shared__ int list[kMaxTopk + 2];
   __shared__ int scratch[2];
@@ -960,19 +963,19 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
   RowState<D> st;
   st.reset();
 
-  const TileCopies<D, W> copies(p, t, smem, wave);
+  const TileCopies<D, W, STEP> copies(p, t, smem, wave);
   // this workgroup's steps of the list's, from a block and an offset in it on
-  const int per = p.bk / kSub, steps = n * per;
+  const int per = p.bk / STEP, steps = n * per;
   const int first = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
   const int last = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
-  int e = first / per, off = (first - e * per) * kSub, buf = 0;
+  int e = first / per, off = (first - e * per) * STEP, buf = 0;
   int blk = __builtin_amdgcn_readfirstlane(list[e]);
   int nxt = list[e + 1];  // (past the last block it may be anything)
   if (first < last) copies.issue(p, blk * p.bk + off, 0, t.tk.limit);
   for (int step = first; step < last;) {
     const int key = blk * p.bk + off;
     ++step;
-    off += kSub;
+    off += STEP;
     if (off == p.bk) {
       off = 0;
       ++e;
@@ -985,7 +988,7 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
     asm volatile("" ::: "memory");
     if (step < last) copies.issue(p, blk * p.bk + off, buf ^ 1, t.tk.limit);
     const char *kt = smem + buf * 2 * TILE;
-    attend_step<D, 2, F16, false, false>(kt, kt + TILE, qf, max(0, t.tk.limit - key), p.scale_log2, st);
+    attend_step<D, STEP / 32, F16, false, false>(kt, kt + TILE, qf, max(0, t.tk.limit - key), p.scale_log2, st);
     buf ^= 1;
   }
   const float l = both_sum(st.l);
@@ -1023,7 +1026,7 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnPar
 // the other as in the tile kernel.
 constexpr int kWindow = 1024;    // blocks whose lists are joined at a time
 constexpr int kMaxGroup = 32;    // tiles: a bit each
-constexpr int kGroupItems = 512; // workgroups that the chip takes in one round, two a unit
+constexpr int kPlaces = 512;     // workgroups that the chip takes in one round, two a unit
 
 template <int D, int W, bool F16>
 __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnParams p) {
@@ -1042,7 +1045,7 @@ __global__ void __launch_bounds__(64 * W, 2) block_attn_group_kernel(BlockAttnPa
   load_query<D>(p, t, r, qf);
   wait_copies<0>();  // (no load of the compiler's own is then pending among the copies)
 
-  const TileCopies<D, W> copies(p, t, smem, wave);
+  const TileCopies<D, W, kSub> copies(p, t, smem, wave);
   const int32_t *src = tile_list(p, t);
   const int64_t row = static_cast<int64_t>(p.Hkv) * p.topk;
   const int last = (t.rows / p.G - 1) / p.bq;  // the group's last tile, whose limit t.tk has
@@ -1634,7 +1637,7 @@ static AttnPlan attn_plan(const pkv_block_attn_args *a) {
     // rounds) 95 / 190, one by one 163 / 181
     const int64_t most = 128 / rows < kMaxGroup ? 128 / rows : kMaxGroup;
     int64_t g = 1;
-    while (g < most && heads * ((tiles + g - 1) / g) > kGroupItems) g = 2 * g < most ? 2 * g : most;
+    while (g < most && heads * ((tiles + g - 1) / g) > kPlaces) g = 2 * g < most ? 2 * g : most;
     s.group = static_cast<int>(g);
   }
   s.tiles = (tiles + s.group - 1) / s.group;
@@ -1657,8 +1660,11 @@ static AttnPlan attn_plan(const pkv_block_attn_args *a) {
     // KV heads of 48 query heads and 15 blocks 16.3 (25.8; 26.5 in pieces of 8), 156
     // tiles of 128 rows and 64 blocks 72 in threes (91), but 200 of 32 blocks 61 in
     // twos (51)
-    const int64_t places = (rows <= 128 ? 512 : 256) / s.items;
+    int64_t places = (rows <= 128 ? kPlaces : kPlaces / 2) / s.items;
     const int64_t pieces = static_cast<int64_t>(a->topk) * (a->block_k / kSub) / 4;
+    // (four a unit in steps of 32 keys: 300 tiles of 64 rows and 64 blocks 87 us in
+    // threes, 104 alone, but 256 of 8 blocks 31 in twos, 18 alone)
+    if (rows <= 64 && places < 3 && pieces >= 3) places = 2 * kPlaces / s.items;
     const int64_t n = places < pieces ? places : pieces;
     if (places >= 3 && n > 1) s.splits = static_cast<int>(n);
   }
@@ -1676,7 +1682,9 @@ static int launch_block_attn(const BlockAttnParams &p, hipStream_t st) {
   }
   if (rows > 32) {
     const int w = rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
-    auto *k = w == 2 ? block_attn_tile_kernel<D, 2, F16> : w == 4 ? block_attn_tile_kernel<D, 4, F16> : block_attn_tile_kernel<D, 8, F16>;
+    auto *k = w == 4 ? block_attn_tile_kernel<D, 4, 64, F16> : block_attn_tile_kernel<D, 8, 64, F16>;
+    if (w == 2)
+      k = p.items * p.splits > kPlaces ? block_attn_tile_kernel<D, 2, 32, F16> : block_attn_tile_kernel<D, 2, 64, F16>;
     hipLaunchKernelGGL(k, dim3(p.items * p.splits), dim3(64 * w), 0, st, p);
     if (const int rc = check_launch("block_attn_tile_kernel")) return rc;
   } else {

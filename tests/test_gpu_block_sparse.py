@@ -331,6 +331,8 @@ ATTEND = [  # q lens, k lens, hkv, G, per_head, topk, bq, bk, causal
     ([120], [5000], 2, 1, True, 40, 120, 64, False), ([1], [9000], 1, 48, False, 80, 1, 64, False),
     ([40, 3], [3000, 0], 1, 6, False, 24, 40, 64, False), ([70], [20000], 1, 2, False, 9, 32, 1024, False),
     ([1, 1], [2500, 130], 1, 128, False, 33, 1, 64, True), ([9], [70000], 1, 16, False, 1024, 9, 64, False),
+    # many tiles of 33 to 64 rows: steps of 32 keys, split or not
+    ([590], [900, ], 1, 40, False, 5, 1, 64, True), ([260], [3000], 1, 33, False, 17, 1, 128, False),
 ]
 
 
