@@ -1024,10 +1024,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_pp_kernel(AttnParams p) {
     rsrc[3] = kRsrcWord3;
     const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)slot)) + dma_lds;
     // m0 is reserved to the compiler, which uses it nowhere else in this
-    // kernel (the listing has no other m0 access)
+    // kernel (the listing has no other m0 access); a load into LDS must not
+    // directly follow its write, and the compiler adds no s_nop in here
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(lds), "v"(voff), "s"(rsrc)
                  : "memory", "m0");
@@ -1453,9 +1454,10 @@ __device__ __attribute__((always_inline)) inline void tail_item(const AttnParams
       const int sw = ckind ? (dpos ^ (4 * (r & 3))) : (dpos ^ (r & 15));
       const int voff = r * row_bytes + 16 * sw;
       const uint32_t lds = lds0 + ch * 4 * kPRow;
+      // (s_nop: a load into LDS must not directly follow the write of m0)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    :
                    : "s"(lds), "v"(voff), "s"(rsrc)
                    : "memory", "m0");
@@ -1496,9 +1498,10 @@ __device__ __attribute__((always_inline)) inline void tail_item(const AttnParams
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int voff = (16 * u + (lane >> 2)) * row_bytes + 64 * (lane & 3);
+      // (s_nop as above)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                    :
                    : "s"(sink0), "v"(voff), "s"(rsrc)
                    : "memory", "m0");
@@ -1734,10 +1737,11 @@ __device__ __attribute__((always_inline)) inline void p3_item(const AttnParams &
     rsrc[3] = kRsrcWord3;
     const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)slot)) + dma_lds;
     // m0 is reserved to the compiler, which uses it nowhere else in this
-    // kernel (the listing has no other m0 access)
+    // kernel (the listing has no other m0 access); a load into LDS must not
+    // directly follow its write, and the compiler adds no s_nop in here
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(lds), "v"(voff), "s"(rsrc)
                  : "memory", "m0");

@@ -622,10 +622,11 @@ __device__ inline void copy_rows(const uint16_t *base, int64_t bytes, uint32_t l
   rsrc[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
   rsrc[3] = 0x00020000;
   // (the copies are inline assembly so that the compiler inserts no wait of its
-  // own for them before LDS reads; every wait for them is explicit)
+  // own for them before LDS reads; every wait for them is explicit.  Nor does it add
+  // the wait state between the write of m0 and a load into LDS, hence s_nop)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
 #pragma clang diagnostic pop
 }
 

@@ -2253,9 +2253,10 @@ __global__ void __launch_bounds__(kUpdThreads)
 #pragma unroll
     for (int m = 0; m < kTok; ++m) {
       const uint32_t lds = ring0 + static_cast<uint32_t>(((r * 4 + wave_s) * kTok + m) * 1024);
+      // (s_nop: a load into LDS must not directly follow the write of m0)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
                    :
                    : "s"(lds), "v"(fo + toff[m]), "s"(srsrc)
                    : "memory", "m0");
