@@ -612,7 +612,9 @@ __device__ inline int v_chunk(int row, int c) { return c ^ (D == 128 ? 4 * (row 
 
 // One wave's copy of 64 / (D / 8) consecutive key rows into LDS at byte
 // address lds (uniform), the chunks in the order that `voff` (this lane's
-// source byte, relative to base) says; rows past `bytes` become zero.
+// source byte, relative to base) says; rows past `bytes` become zero.  FIRST: the
+// first copy with this base and these bytes.
+template <bool FIRST>
 __device__ inline void copy_rows(const uint16_t *base, int64_t bytes, uint32_t lds, int voff) {
   const uint64_t addr = reinterpret_cast<uint64_t>(base);
   i32x4 rsrc;
@@ -621,13 +623,25 @@ __device__ inline void copy_rows(const uint16_t *base, int64_t bytes, uint32_t l
   rsrc[1] = __builtin_amdgcn_readfirstlane(static_cast<int>((addr >> 32) & 0xffffu));
   rsrc[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
   rsrc[3] = 0x00020000;
-  // (the copies are inline assembly so that the compiler inserts no wait of its
-  // own for them before LDS reads; every wait for them is explicit.  Nor does it add
-  // the wait state between the write of m0 and a load into LDS, hence s_nop)
+  // The copies are inline assembly so that the compiler inserts no wait of its
+  // own for them before LDS reads; every wait for them is explicit.  Nor does it
+  // add wait states: one is due between the write of m0 and a load into LDS, five
+  // between a vector instruction's write of a scalar register (v_readfirstlane
+  // above) and a memory instruction that reads it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(rsrc), "n"(FIRST ? 3 : 0)
+               : "memory", "m0");
 #pragma clang diagnostic pop
+}
+// copy(i, whether it is the first) for i < COPIES
+template <int COPIES, typename F>
+__device__ inline void copy_each(F copy) {
+  copy(0, std::true_type());
+#pragma unroll
+  for (int i = 1; i < COPIES; ++i) copy(i, std::false_type());
 }
 
 // The valid entries of a tile's list, each once, into LDS: list[0 .. return).
@@ -918,11 +932,10 @@ struct TileCopies {
     const int left = max(0, min(STEP, limit - key));
     const int64_t off = left > 0 ? key * p.kv_tok : 0;
     const uint32_t dst = lds + buf * 2 * TILE;
-#pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      copy_rows(k + off, static_cast<int64_t>(left) * row_bytes, dst + i * RPC * ROW, kvoff[i]);
-      copy_rows(v + off, static_cast<int64_t>(left) * row_bytes, dst + i * RPC * ROW + TILE, vvoff[i]);
-    }
+    copy_each<COPIES>([&](int i, auto first) {
+      copy_rows<decltype(first)::value>(k + off, static_cast<int64_t>(left) * row_bytes, dst + i * RPC * ROW, kvoff[i]);
+      copy_rows<decltype(first)::value>(v + off, static_cast<int64_t>(left) * row_bytes, dst + i * RPC * ROW + TILE, vvoff[i]);
+    });
   }
 };
 
@@ -1200,12 +1213,11 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 1) block_attn_small_kernel(B
   auto issue = [&](int key, int buf) {
     const int left = max(0, min(32, t.tk.limit - key));
     const int64_t off = left > 0 ? key * p.kv_tok : 0;
-#pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
+    copy_each<COPIES>([&](int i, auto first) {
       const uint32_t at = lds0 + buf * 2 * TILE + i * RPC * ROW;
-      copy_rows(kp + off, static_cast<int64_t>(left) * row_bytes, at, kvoff[i]);
-      copy_rows(vp + off, static_cast<int64_t>(left) * row_bytes, at + TILE, vvoff[i]);
-    }
+      copy_rows<decltype(first)::value>(kp + off, static_cast<int64_t>(left) * row_bytes, at, kvoff[i]);
+      copy_rows<decltype(first)::value>(vp + off, static_cast<int64_t>(left) * row_bytes, at + TILE, vvoff[i]);
+    });
   };
   // this wave's steps: every (4 * splits)-th 32 keys of the list, as an entry and an
   // offset in its block

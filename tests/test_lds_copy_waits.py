@@ -130,7 +130,7 @@ def test_what_counts():
 
 
 @pytest.mark.skipif(not os.path.exists(OBJDUMP), reason="no disassembler")
-@pytest.mark.parametrize("what", [M0])
+@pytest.mark.parametrize("what", [M0, "descriptor"])
 def test_copies_into_lds_wait(what, tmp_path):
     copies, bad = 0, []
     for text in listing(tmp_path):
