@@ -431,6 +431,14 @@ int pkv_rotary(const pkv_rotary_args *args, pkv_stream_t stream);
  * dtype bf16 or fp16.  causal (block_q 1 only): query i of a sequence of n sees
  * its keys up to keys - n + i. */
 
+/* causal of pkv_block_select_args.  The block that holds a token's last key may
+ * hold later keys, which its mean then covers: PKV_CAUSAL takes that block
+ * whatever its score, as if recent_blocks were 1 at least (the sink blocks come
+ * first where topk has room for no more), so that the lists depend on no later
+ * key.  PKV_CAUSAL_RANKED ranks it like the others, for means that hold no later
+ * keys. */
+enum pkv_causal { PKV_NOT_CAUSAL = 0, PKV_CAUSAL = 1, PKV_CAUSAL_RANKED = 2 };
+
 /* The mean of every block's keys, in fp32: means [rows, KV heads, head_dim]
  * (one head a row with kv_per_head).  num_seqs key sequences.  last 0: rows
  * without keys become zero.  last n > 0: only the blocks that hold one of a
@@ -466,7 +474,8 @@ typedef struct pkv_block_select_args {
   int64_t q_tok_stride, q_head_stride;
   int32_t num_batches, num_heads_q, num_heads_kv, head_dim, kv_per_head;
   int32_t max_seqlen_q, max_seqlen_k;
-  int32_t block_q, block_k, topk, sink_blocks, recent_blocks, causal;
+  int32_t block_q, block_k, topk, sink_blocks, recent_blocks;
+  int32_t causal; /* enum pkv_causal */
   int32_t dtype;
 } pkv_block_select_args;
 

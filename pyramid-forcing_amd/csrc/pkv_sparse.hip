@@ -1485,6 +1485,8 @@ static int check_select(const pkv_block_select_args *a) {
   if (const int rc = check_block(a->head_dim, a->block_k, a->dtype, "block_select")) return rc;
   if (const int rc = check_tiles(a->num_heads_q, a->num_heads_kv, a->block_q, a->topk, a->causal, "block_select"))
     return rc;
+  if (a->causal < PKV_NOT_CAUSAL || a->causal > PKV_CAUSAL_RANKED)
+    return fail(PKV_ERR_INVALID, "block_select: causal %d", a->causal);
   if (a->sink_blocks < 0 || a->recent_blocks < 0 || static_cast<int64_t>(a->sink_blocks) + a->recent_blocks > a->topk)
     return fail(PKV_ERR_INVALID, "block_select: %d sink and %d recent blocks of %d", a->sink_blocks, a->recent_blocks,
                 a->topk);
@@ -1603,6 +1605,9 @@ extern "C" int pkv_block_select(const pkv_block_select_args *a, void *workspace,
   p.nb = static_cast<int>(s.nb);
   p.bq = a->block_q; p.bk = a->block_k; p.topk = a->topk; p.sink = a->sink_blocks; p.recent = a->recent_blocks;
   p.causal = a->causal ? 1 : 0;
+  // a token's own block, the last that it chooses from, is taken, not scored: its
+  // mean covers later keys
+  if (a->causal == PKV_CAUSAL && p.recent < 1) p.recent = 1;
   p.sums = s.sums_bytes ? static_cast<double *>(workspace) : nullptr;
   p.keys = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + s.sums_bytes);
   hipStream_t st = as_stream(stream);

@@ -945,7 +945,7 @@ static int64_t kv_heads_of(const Tensor &kv, int64_t cu_entries, int64_t B, cons
 
 static Tensor block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int64_t max_seqlen_q,
                            int64_t max_seqlen_k, int64_t topk, int64_t block_q, int64_t block_k, int64_t sink_blocks,
-                           int64_t recent_blocks, bool causal, c10::optional<Tensor> seqlens_k) {
+                           int64_t recent_blocks, bool causal, c10::optional<Tensor> seqlens_k, bool rank_own) {
   const char *who = "block_select";
   TORCH_CHECK(q.is_cuda() && q.dim() == 3, who, ": q must be a GPU tensor [total_q, heads, head_dim]");
   check_rows(q, q, who, "q");
@@ -982,7 +982,7 @@ static Tensor block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor c
   a.topk = to_i32(topk, who, "topk");
   a.sink_blocks = to_i32(sink_blocks, who, "sink_blocks");
   a.recent_blocks = to_i32(recent_blocks, who, "recent_blocks");
-  a.causal = causal ? 1 : 0;
+  a.causal = !causal ? PKV_NOT_CAUSAL : rank_own ? PKV_CAUSAL_RANKED : PKV_CAUSAL;
   a.dtype = dtype_code(q, false, who);
   c10::DeviceGuard guard(q.device());
   Tensor lists = at::empty({q.size(0) / block_q + B, Hkv, topk}, q.options().dtype(at::kInt));
@@ -1530,7 +1530,7 @@ static Tensor block_means(Tensor k, Tensor cu, int64_t block_k, int64_t, c10::op
 }
 static void block_means_(Tensor, Tensor, Tensor, int64_t, int64_t, int64_t, c10::optional<Tensor>) {}
 static Tensor block_select(Tensor q, Tensor means, Tensor cu_q, Tensor cu_k, int64_t, int64_t, int64_t topk,
-                           int64_t block_q, int64_t, int64_t, int64_t, bool, c10::optional<Tensor>) {
+                           int64_t block_q, int64_t, int64_t, int64_t, bool, c10::optional<Tensor>, bool) {
   const int64_t B = cu_q.numel() - 1;
   return at::empty({q.size(0) / block_q + B, adahead::kv_heads_of(means, cu_k.numel(), B, "block_select"), topk},
                    q.options().dtype(at::kInt));
@@ -1680,7 +1680,7 @@ TORCH_LIBRARY(adahead, m) {
         "Tensor? seqlens_k=None) -> ()");
   m.def("block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, "
         "int max_seqlen_k, int topk, int block_q, int block_k, int sink_blocks=0, int recent_blocks=0, "
-        "bool causal=False, Tensor? seqlens_k=None) -> Tensor");
+        "bool causal=False, Tensor? seqlens_k=None, bool rank_own=False) -> Tensor");
   m.def("block_sparse_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, "
         "int max_seqlen_q, Tensor lists, float softmax_scale, int block_q, int block_k, bool causal=False, "
         "bool return_lse=False, Tensor? seqlens_k=None) -> Tensor[]");

@@ -64,16 +64,20 @@ def block_means(k, cu_seqlens_k, block_k=64, *, max_seqlen_k=0, seqlens_k=None, 
 
 
 def block_select(q, means, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, topk, *, block_q=128, block_k=64,
-                 sink_blocks=0, recent_blocks=0, causal=False, seqlens_k=None):
+                 sink_blocks=0, recent_blocks=0, causal=False, seqlens_k=None, rank_own=False):
     """The blocks that each tile attends to, [tile rows, kv_heads, topk] int32,
     ascending and padded with -1.  A block's score is the product of the tile's
     summed queries with its mean, summed in 64 bits and rounded to fp32 (ties:
     the lower index; NaN counts as -inf).  Keys past max_seqlen_k are not
     considered, and tiles past max_seqlen_q get no block.  causal (block_q 1):
-    token i of n chooses from the blocks that hold its keys up to keys - n + i."""
+    token i of n chooses from the blocks that hold its keys up to keys - n + i.
+    The last of them is taken whatever its score, as by recent_blocks 1: its mean
+    may cover later keys, on which no choice depends so (where sink_blocks is topk
+    there is no room for it).  rank_own: that block is ranked like the others, for
+    means that hold no later keys."""
     return _ops.ops().block_select(q, means, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k), int(topk),
                                    int(block_q), int(block_k), int(sink_blocks), int(recent_blocks), bool(causal),
-                                   seqlens_k)
+                                   seqlens_k, bool(rank_own))
 
 
 def block_sparse_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, lists, *, block_q=128, block_k=64,
@@ -94,7 +98,8 @@ def block_sparse_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, li
 
 def sparse_ragged_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, sparse: BlockSparse, *,
                             softmax_scale=None, causal=False, seqlens_k=None, means=None):
-    """Means (unless given), selection and attention in a row."""
+    """Means (unless given), selection and attention in a row.  causal: no result
+    depends on a later key, through the choice of blocks either."""
     if means is None:
         means = block_means(k, cu_seqlens_k, sparse.block_k, max_seqlen_k=max_seqlen_k, seqlens_k=seqlens_k)
     lists = block_select(q, means, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, sparse.topk,

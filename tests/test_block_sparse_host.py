@@ -197,3 +197,8 @@ def test_meta_shapes():
     r = ops.rotary(q, q[:, :2], pos, f, [16], True, 1.0, False)
     assert [t.shape for t in r] == [q.shape, (10, 2, 128)]
     assert len(ops.rotary(q, None, pos, f, [16], True, 1.0, False)) == 1
+
+
+@pytest.mark.parametrize("causal", [-1, 3])
+def test_selection_refuses_other_causal_forms(causal):
+    _refused(A.lib().pkv_block_select(ctypes.byref(_select(causal=causal, block_q=1)), FAKE, 1 << 40, None))

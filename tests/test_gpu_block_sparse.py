@@ -737,3 +737,55 @@ def test_arguments_are_sound():
     a = _args()
     bs.block_sparse_attention(a["q"], a["k"], a["v"], a["cq"], a["ck"], a["mq"], a["lists"], block_q=4)
     bs.block_select(a["q"], a["means"], a["cq"], a["ck"], a["mq"], a["mk"], 3, block_q=4)
+
+
+# ---------------------------------------------------------------------------
+# causal choices
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n,hkv,G,topk,sink,bk", [(640, 1, 2, 3, 0, 64), (1000, 2, 4, 4, 1, 128), (300, 2, 8, 1, 0, 64),
+                                                  (9000, 1, 1, 5, 0, 64), (500, 1, 1, 2, 2, 64)])
+def test_causal_choice_sees_no_later_keys(n, hkv, G, topk, sink, bk):
+    """Keys after token i, and what they do to its own block's mean, leave the
+    lists and results of the tokens up to i as they were, with no recent block
+    asked for too; and a token decoded by itself chooses as it does in the prompt."""
+    tokens = min(n, 700)  # (a prompt, or the last part of one over a longer context)
+    q, k, v = rnd(tokens, hkv * G, 64), rnd(n, hkv, 64), rnd(n, hkv, 64)
+    sparse = bs.BlockSparse(topk=topk, block_q=1, block_k=bk, sink_blocks=sink)
+
+    def both(kk):
+        means = bs.block_means(kk, cu([n]), bk)
+        return (bs.block_select(q, means, cu([tokens]), cu([n]), tokens, n, topk, block_q=1, block_k=bk, sink_blocks=sink,
+                                causal=True),
+                bs.sparse_ragged_attention(q, kk, v, cu([tokens]), cu([n]), tokens, n, sparse, causal=True))
+
+    lists, out = both(k)
+    for last in (n - 1, n - 60, n - bk - 7, n - tokens + 130):  # the last key that stays
+        i = last - (n - tokens)
+        if not 0 <= i < tokens:
+            continue
+        for size in (30.0, -30.0):
+            kk = k.clone()
+            kk[last + 1:] = (rnd(n - last - 1, hkv, 64) + q[i].view(hkv, G, 64).sum(dim=1)) * size
+            l2, o2 = both(kk)
+            assert torch.equal(l2[:i + 1], lists[:i + 1]) and torch.equal(o2[:i + 1], out[:i + 1])
+        used = torch.tensor([last + 1], dtype=torch.int32, device=DEV)
+        one = bs.block_select(q[i:i + 1], bs.block_means(k, cu([n]), bk, seqlens_k=used), cu([1]), cu([n]), 1, n, topk,
+                              block_q=1, block_k=bk, sink_blocks=sink, causal=True, seqlens_k=used)
+        assert torch.equal(one[0], lists[i])
+    # the list of a token: its own block, and the best of those before
+    j = lists[tokens - 1].cpu()
+    assert ((j == (n - 1) // bk).any(dim=-1) | (sink >= topk)).all()
+
+
+def test_own_blocks_ranked():
+    """rank_own: the formula as it stands, later keys and all."""
+    for n, hkv, G, topk, sink in ((640, 1, 2, 3, 0), (300, 2, 8, 1, 0), (500, 1, 1, 1, 1)):
+        q, means = rnd(n, hkv * G, 64), torch.randn(n // 64 + 1, hkv, 64, device=DEV)
+        got = bs.block_select(q, means, cu([n]), cu([n]), n, n, topk, block_q=1, sink_blocks=sink, causal=True, rank_own=True)
+        want = _select_ref(q, means, [n], [n], hkv, False, topk, 1, 64, sink, 0, True)
+        assert np.array_equal(got.cpu().numpy(), want)
+        # the own block taken: the formula with one recent block
+        if topk > sink:
+            got = bs.block_select(q, means, cu([n]), cu([n]), n, n, topk, block_q=1, sink_blocks=sink, causal=True)
+            want = _select_ref(q, means, [n], [n], hkv, False, topk, 1, 64, sink, 1, True)
+            assert np.array_equal(got.cpu().numpy(), want)
