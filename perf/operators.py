@@ -357,10 +357,12 @@ def run(state):
         if kind == "means":
             return block_sparse.block_means(state["k"], state["cu_k"], case["block"], max_seqlen_k=state["k_max"])
         if kind == "select":
+            # the formula ranks a token's own block by its mean like the others
+            ranked = dict(rank_own=True) if case["causal"] and not case["recent"] else {}
             return block_sparse.block_select(state["q"], state["means"], state["cu_q"], state["cu_k"], state["q_max"],
                                              state["k_max"], case["topk"], block_q=case["block_q"],
                                              block_k=case["block"], sink_blocks=case["sink"],
-                                             recent_blocks=case["recent"], causal=case["causal"])
+                                             recent_blocks=case["recent"], causal=case["causal"], **ranked)
         out = block_sparse.block_sparse_attention(state["q"], state["k"], state["v"], state["cu_q"], state["cu_k"],
                                                   state["q_max"], state["lists"], block_q=case["block_q"],
                                                   block_k=case["block"], causal=case["causal"], return_lse=case["lse"])
