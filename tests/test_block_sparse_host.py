@@ -202,3 +202,24 @@ def test_meta_shapes():
 @pytest.mark.parametrize("causal", [-1, 3])
 def test_selection_refuses_other_causal_forms(causal):
     _refused(A.lib().pkv_block_select(ctypes.byref(_select(causal=causal, block_q=1)), FAKE, 1 << 40, None))
+
+
+# ---- derivatives ------------------------------------------------------------------
+def test_rotary_keeps_forward_derivatives():
+    """On tensors without storage: a tangent comes out where one goes in."""
+    from torch.autograd import forward_ad as fw
+    m = dict(device="meta")
+    q, k = torch.empty(10, 8, 64, **m), torch.empty(10, 2, 64, **m)
+    pos, f = torch.empty(10, dtype=torch.int64, **m), torch.empty(32, dtype=torch.float64, **m)
+    with fw.dual_level():
+        dual = lambda x: fw.make_dual(x, torch.empty_like(x))
+        assert fw.unpack_dual(rope.rotary(dual(q), pos, f)).tangent.shape == q.shape
+        a, b = (fw.unpack_dual(x) for x in rope.rotary(dual(q), pos, f, k=dual(k)))
+        assert a.tangent.shape == q.shape and b.tangent.shape == k.shape
+        assert fw.unpack_dual(rope.rotary(q, pos, f, k=dual(k))[1]).tangent.shape == k.shape
+    y, t = torch.func.jvp(lambda x: rope.rotary(x, pos, f), (q,), (torch.empty_like(q),))
+    assert y.shape == t.shape == q.shape
+    assert torch.func.grad(lambda x: rope.rotary(x, pos, f).sum())(q).shape == q.shape
+    assert torch.func.vmap(lambda x: rope.rotary(x, pos, f))(torch.empty(3, 10, 8, 64, **m)).shape == (3, 10, 8, 64)
+    with pytest.raises(RuntimeError):
+        rope.rotary(q, pos, f.requires_grad_())

@@ -261,3 +261,75 @@ def test_rotary_refuses(name):
     kw.update(REFUSED[name]())
     with pytest.raises(RuntimeError):
         rope.rotary(kw.pop("q"), kw.pop("positions"), kw.pop("freqs"), **kw)
+
+
+# ---- forward derivatives, batches --------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF], ids=str)
+def test_rotary_forward_derivative(dtype):
+    """The rotation is linear: the derivative along a tangent is the rotated
+    tangent, for q, for k, and for the one of them that has one."""
+    from torch.autograd import forward_ad as fw
+    f, pos = rope.rotary_frequencies(48, device=DEV)[0], torch.randint(0, 9999, (31,), device=DEV)
+    q, tq = (torch.randn(31, 6, 64, device=DEV).to(dtype) for _ in range(2))
+    k, tk = (torch.randn(31, 2, 64, device=DEV).to(dtype) for _ in range(2))
+    kw = dict(interleaved=False, scale=1.5)
+    args = (pos, f, (24,), False, 1.5, False)
+    with fw.dual_level():
+        out = fw.unpack_dual(rope.rotary(fw.make_dual(q, tq), pos, f, **kw))
+        assert torch.equal(out.primal, rope.rotary(q, pos, f, **kw))
+        _check(out.tangent, tq, *args)
+        a, b = (fw.unpack_dual(x) for x in rope.rotary(fw.make_dual(q, tq), pos, f, k=fw.make_dual(k, tk), **kw))
+        _check(a.tangent, tq, *args)
+        _check(b.tangent, tk, *args)
+        a, b = (fw.unpack_dual(x) for x in rope.rotary(q, pos, f, k=fw.make_dual(k, tk), **kw))
+        assert a.tangent is None or not a.tangent.any()
+        _check(b.tangent, tk, *args)
+        a, b = (fw.unpack_dual(x) for x in rope.rotary(fw.make_dual(q, tq), pos, f, k=k, **kw))
+        assert b.tangent is None or not b.tangent.any()
+        _check(a.tangent, tq, *args)
+    y, t = torch.func.jvp(lambda x: rope.rotary(x, pos, f, **kw), (q,), (tq,))
+    assert torch.equal(y, rope.rotary(q, pos, f, **kw))
+    _check(t, tq, *args)
+    # forwards over backwards: the derivative of a gradient
+    if dtype == F32:
+        loss = lambda x: (rope.rotary(x, pos, f, **kw) ** 3).sum() / 3
+        g, h = torch.func.jvp(torch.func.grad(loss), (q,), (tq,))
+        y, t = rope.rotary(q, pos, f, **kw).double(), rope.rotary(tq, pos, f, **kw).double()
+        # What is rotated back is rounded before: torch's (1/3) * (3 * y^2) for y^2
+        # takes four roundings of 2^-24 (y^2, times 3, 1/3, the product), its
+        # (1/3) * (3 * (2 y)) * t for 2 y t four (times 3, 1/3, two products); in
+        # another order or with the factors apart at most four more.  A pair's
+        # rounded values are off by 8 * 2^-24 of each, which turns into 8 * 2^-24 of
+        # s (|u| + |w|): two thirds of e.
+        for got, x in ((g, y * y), (h, 2 * y * t)):
+            want, e = _ref(x, pos, f, (24,), False, 1.5, True)
+            # (columns 48 on, where e is 0, are copied with the 8 * 2^-24 of their own)
+            own = torch.where(torch.arange(64, device=DEV) < 48, 1, 8) * 2.0 ** -24
+            assert ((got.double() - want).abs() <= e * (1 + 8 / 12) + own * (want.abs() + 2 * e)).all()
+
+
+def test_rotary_of_batches():
+    """torch.func.vmap over q, over q, k and positions, and over a gradient."""
+    f = rope.rotary_frequencies(64, device=DEV)[0]
+    pos = torch.randint(0, 9999, (5, 31), device=DEV)
+    q, k = torch.randn(5, 31, 4, 64, device=DEV).to(BF), torch.randn(31, 5, 2, 64, device=DEV).to(BF)
+    got = torch.func.vmap(lambda x: rope.rotary(x, pos[0], f))(q)
+    assert torch.equal(got, torch.stack([rope.rotary(x, pos[0], f) for x in q]))
+    a, b = torch.func.vmap(lambda x, y, p: rope.rotary(x, p, f, k=y), in_dims=(0, 1, 0))(q, k, pos)
+    want = [rope.rotary(q[i], pos[i], f, k=k[:, i]) for i in range(5)]
+    assert torch.equal(a, torch.stack([w[0] for w in want])) and torch.equal(b, torch.stack([w[1] for w in want]))
+    g = torch.randn(5, 31, 4, 64, device=DEV).to(BF)
+    grads = torch.func.vmap(lambda x, p, y: torch.func.vjp(lambda z: rope.rotary(z, p, f), x)[1](y)[0])(q, pos, g)
+    assert torch.equal(grads, torch.stack([rope.rotary(g[i], pos[i], f, inverse=True) for i in range(5)]))
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.func.vmap(lambda x, y: rope.rotary(x, pos[0], y))(q, f.expand(5, 32))
+
+
+def test_rotary_refuses_frequencies_that_want_gradients():
+    f, pos = rope.rotary_frequencies(64, device=DEV)[0].requires_grad_(), torch.zeros(3, dtype=torch.int64, device=DEV)
+    q = torch.randn(3, 2, 64, device=DEV)
+    for x in (q, q.clone().requires_grad_()):
+        with pytest.raises((RuntimeError, ValueError)):
+            rope.rotary(x, pos, f)
+    with torch.no_grad():
+        assert torch.equal(rope.rotary(q, pos, f), q)
