@@ -889,18 +889,20 @@ static void run_block_means(const Tensor &means, const Tensor &k, const Tensor &
   pkv_check(pkv_block_means(&a, stream_for(k)), who);
 }
 
-static void check_means_args(const Tensor &k, const Tensor &cu, int64_t block_k, const char *who) {
+static void check_means_args(const Tensor &k, const Tensor &cu, const char *who) {
   TORCH_CHECK(k.is_cuda(), who, ": tensors must be on the GPU");
   dtype_code(k, false, who);
-  TORCH_CHECK(k.dim() == 2 || k.dim() == 3, who, ": k must be [total_k, D] or [total_k, heads, D]");
   TORCH_CHECK(k.dim() == 2 || k.size(1) > 0, who, ": k must have heads");
   check_rows(k, k, who, "k");
   check_aligned(k, who, "k");
   check_cu(cu, k, who, "cu_seqlens_k");
-  TORCH_CHECK(block_k > 0, who, ": block_k must be positive");
 }
 
-static std::vector<int64_t> means_shape(const Tensor &k, int64_t seqs, int64_t block_k) {
+static std::vector<int64_t> means_shape(const Tensor &k, const Tensor &cu, int64_t block_k, const char *who) {
+  TORCH_CHECK(k.dim() == 2 || k.dim() == 3, who, ": k must be [total_k, D] or [total_k, heads, D]");
+  TORCH_CHECK(cu.dim() == 1 && cu.numel() >= 1, who, ": cu_seqlens_k must have at least one entry");
+  TORCH_CHECK(block_k > 0, who, ": block_k must be positive");
+  const int64_t seqs = cu.numel() - 1;
   std::vector<int64_t> s = {k.size(0) / block_k + seqs};
   if (k.dim() == 3) s.push_back(k.size(1));
   s.push_back(k.size(-1));
@@ -910,9 +912,10 @@ static std::vector<int64_t> means_shape(const Tensor &k, int64_t seqs, int64_t b
 static Tensor block_means(Tensor k, Tensor cu_seqlens_k, int64_t block_k, int64_t max_seqlen_k,
                           c10::optional<Tensor> seqlens_k) {
   const char *who = "block_means";
-  check_means_args(k, cu_seqlens_k, block_k, who);
+  const std::vector<int64_t> shape = means_shape(k, cu_seqlens_k, block_k, who);
+  check_means_args(k, cu_seqlens_k, who);
   c10::DeviceGuard guard(k.device());
-  Tensor means = at::empty(means_shape(k, cu_seqlens_k.numel() - 1, block_k), k.options().dtype(at::kFloat));
+  Tensor means = at::empty(shape, k.options().dtype(at::kFloat));
   run_block_means(means, k, cu_seqlens_k, block_k, 0, max_seqlen_k, seqlens_k, who);
   return means;
 }
@@ -920,8 +923,8 @@ static Tensor block_means(Tensor k, Tensor cu_seqlens_k, int64_t block_k, int64_
 static void block_means_(Tensor means, Tensor k, Tensor cu_seqlens_k, int64_t block_k, int64_t last,
                          int64_t max_seqlen_k, c10::optional<Tensor> seqlens_k) {
   const char *who = "block_means_";
-  check_means_args(k, cu_seqlens_k, block_k, who);
-  const std::vector<int64_t> shape = means_shape(k, cu_seqlens_k.numel() - 1, block_k);
+  const std::vector<int64_t> shape = means_shape(k, cu_seqlens_k, block_k, who);
+  check_means_args(k, cu_seqlens_k, who);
   TORCH_CHECK(means.device() == k.device() && means.scalar_type() == at::kFloat && means.is_contiguous() &&
                   means.sizes() == at::IntArrayRef(shape),
               who, ": means must be contiguous float32 ", at::IntArrayRef(shape), " on ", k.device());
@@ -943,6 +946,15 @@ static int64_t kv_heads_of(const Tensor &kv, int64_t cu_entries, int64_t B, cons
   return (cu_entries - 1) / B;
 }
 
+// [tile rows, KV heads, topk]
+static std::vector<int64_t> lists_shape(const Tensor &q, const Tensor &cu_q, int64_t kv_heads, int64_t block_q,
+                                        int64_t topk, const char *who) {
+  TORCH_CHECK(q.dim() == 3, who, ": q must be [total_q, heads, head_dim]");
+  TORCH_CHECK(cu_q.dim() == 1 && cu_q.numel() >= 1, who, ": cu_seqlens_q must have at least one entry");
+  TORCH_CHECK(block_q > 0 && topk > 0, who, ": block_q and topk must be positive");
+  return {q.size(0) / block_q + cu_q.numel() - 1, kv_heads, topk};
+}
+
 static Tensor block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int64_t max_seqlen_q,
                            int64_t max_seqlen_k, int64_t topk, int64_t block_q, int64_t block_k, int64_t sink_blocks,
                            int64_t recent_blocks, bool causal, c10::optional<Tensor> seqlens_k, bool rank_own) {
@@ -958,7 +970,8 @@ static Tensor block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor c
               who, ": means must be contiguous float32 [rows, (heads,) head_dim] on ", q.device());
   check_aligned(means, who, "means");
   const int64_t Hkv = kv_heads_of(means, S + 1, B, who);
-  TORCH_CHECK(block_q > 0 && block_k > 0 && topk > 0, who, ": block_q, block_k and topk must be positive");
+  const std::vector<int64_t> shape = lists_shape(q, cu_seqlens_q, Hkv, block_q, topk, who);
+  TORCH_CHECK(block_k > 0, who, ": block_k must be positive");
   TORCH_CHECK(Hkv > 0 && means.size(0) >= S, who, ": means has too few rows for ", S, " sequences");
   pkv_block_select_args a{};
   a.q = reinterpret_cast<const uint16_t *>(q.data_ptr());
@@ -985,7 +998,7 @@ static Tensor block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor c
   a.causal = !causal ? PKV_NOT_CAUSAL : rank_own ? PKV_CAUSAL_RANKED : PKV_CAUSAL;
   a.dtype = dtype_code(q, false, who);
   c10::DeviceGuard guard(q.device());
-  Tensor lists = at::empty({q.size(0) / block_q + B, Hkv, topk}, q.options().dtype(at::kInt));
+  Tensor lists = at::empty(shape, q.options().dtype(at::kInt));
   a.lists = lists.data_ptr<int32_t>();
   const int64_t need = pkv_block_select_workspace_size(&a);
   Tensor ws;
@@ -1526,14 +1539,14 @@ static std::vector<Tensor> rotary(Tensor q, c10::optional<Tensor> k, Tensor, Ten
   return out;
 }
 static Tensor block_means(Tensor k, Tensor cu, int64_t block_k, int64_t, c10::optional<Tensor>) {
-  return at::empty(adahead::means_shape(k, cu.numel() - 1, block_k), k.options().dtype(at::kFloat));
+  return at::empty(adahead::means_shape(k, cu, block_k, "block_means"), k.options().dtype(at::kFloat));
 }
 static void block_means_(Tensor, Tensor, Tensor, int64_t, int64_t, int64_t, c10::optional<Tensor>) {}
 static Tensor block_select(Tensor q, Tensor means, Tensor cu_q, Tensor cu_k, int64_t, int64_t, int64_t topk,
                            int64_t block_q, int64_t, int64_t, int64_t, bool, c10::optional<Tensor>, bool) {
-  const int64_t B = cu_q.numel() - 1;
-  return at::empty({q.size(0) / block_q + B, adahead::kv_heads_of(means, cu_k.numel(), B, "block_select"), topk},
-                   q.options().dtype(at::kInt));
+  const char *who = "block_select";
+  const int64_t Hkv = adahead::kv_heads_of(means, cu_k.numel(), cu_q.numel() - 1, who);
+  return at::empty(adahead::lists_shape(q, cu_q, Hkv, block_q, topk, who), q.options().dtype(at::kInt));
 }
 static std::vector<Tensor> block_sparse_attention(Tensor q, Tensor, Tensor, Tensor, Tensor, int64_t, Tensor, double,
                                                   int64_t, int64_t, bool, bool lse, c10::optional<Tensor>) {

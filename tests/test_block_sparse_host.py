@@ -223,3 +223,20 @@ def test_rotary_keeps_forward_derivatives():
     assert torch.func.vmap(lambda x: rope.rotary(x, pos, f))(torch.empty(3, 10, 8, 64, **m)).shape == (3, 10, 8, 64)
     with pytest.raises(RuntimeError):
         rope.rotary(q, pos, f.requires_grad_())
+
+
+@pytest.mark.parametrize("block", [0, -64])
+def test_meta_refusals(block):
+    """Shapes of no block size raise (a division by zero would end the process)."""
+    m = dict(device="meta")
+    ops = _ops.ops()
+    q, k = torch.empty(10, 8, 128, dtype=torch.bfloat16, **m), torch.empty(100, 2, 128, dtype=torch.bfloat16, **m)
+    cu, means = torch.empty(3, dtype=torch.int32, **m), torch.empty(3, 2, 128, **m)
+    none = torch.empty(0, dtype=torch.int32, **m)
+    for call in (lambda: ops.block_means(k, cu, block), lambda: ops.block_means(k[0, 0], cu, 64),
+                 lambda: ops.block_means(k, none, 64), lambda: ops.block_select(q, means, cu, cu, 5, 50, 3, block, 64),
+                 lambda: ops.block_select(q, means, cu, cu, 5, 50, block, 4, 64),
+                 lambda: ops.block_select(q[0], means, cu, cu, 5, 50, 3, 4, 64),
+                 lambda: ops.block_select(q, means, none, none, 5, 50, 3, 4, 64)):
+        with pytest.raises(RuntimeError):
+            call()
