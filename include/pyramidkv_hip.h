@@ -440,8 +440,8 @@ int pkv_rotary(const pkv_rotary_args *args, pkv_stream_t stream);
 enum pkv_causal { PKV_NOT_CAUSAL = 0, PKV_CAUSAL = 1, PKV_CAUSAL_RANKED = 2 };
 
 /* The mean of every block's keys, in fp32: means [rows, KV heads, head_dim]
- * (one head a row with kv_per_head).  num_seqs key sequences.  last 0: rows
- * without keys become zero.  last n > 0: only the blocks that hold one of a
+ * (one head a row with kv_per_head).  num_seqs key sequences; with none nothing
+ * is written.  last 0: rows without keys become zero.  last n > 0: only the blocks that hold one of a
  * sequence's last n keys are written.  max_seqlen_k: a bound of a sequence's
  * keys that sizes the launch (0: unknown). */
 typedef struct pkv_block_means_args {
@@ -461,8 +461,9 @@ int pkv_block_means(const pkv_block_means_args *args, pkv_stream_t stream);
  * the product of the tile's summed query rows with the block's mean, the
  * sums in 64 bits and the product rounded to fp32 (ties: the lower index; NaN
  * counts as -inf), the first sink_blocks and last recent_blocks always among
- * them; ascending, padded with -1.  Rows that are no tile's are -1.  Blocks past
- * max_seqlen_k keys are not considered, tiles past max_seqlen_q have none.
+ * them; ascending, padded with -1.  Rows that are no tile's are -1 (with no
+ * batches nothing is written).  Blocks past max_seqlen_k keys are not considered,
+ * tiles past max_seqlen_q have none.
  * The workspace (pkv_block_select_workspace_size bytes, no initialisation)
  * must not be shared by calls that may overlap. */
 typedef struct pkv_block_select_args {

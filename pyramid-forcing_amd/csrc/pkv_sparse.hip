@@ -85,14 +85,15 @@ __global__ void __launch_bounds__(256) block_means_kernel(MeansParams p) {
   const int64_t first = begin / p.bk + s;
   // the rows up to the next sequence's, the last sequence's up to the end
   const int64_t end = s + 1 < p.S ? seq_span(p.cu, s + 1, p.total_k).begin / p.bk + s + 1 : p.total_rows;
-  const int from = p.last > 0 ? max(0, n - p.last) / p.bk : 0;
+  // (the first sequence's also zeroes the rows before it)
+  const int64_t from = p.last > 0 ? max(0, n - p.last) / p.bk : s == 0 ? -first : 0;
   const int64_t to = p.last > 0 ? (n + p.bk - 1) / p.bk : end - first;
   const int lane = threadIdx.x & 63, col = 8 * (lane % LPR), sub = lane / LPR;
   const int64_t stride = static_cast<int64_t>(p.chunks) * 4;
-  for (int64_t w = static_cast<int64_t>(from) * p.H + chunk * 4 + (threadIdx.x >> 6); w < to * p.H; w += stride) {
-    const int64_t j = w / p.H;
-    const int h = static_cast<int>(w - j * p.H);
-    const int64_t left = n - j * p.bk;
+  for (int64_t w = chunk * 4 + (threadIdx.x >> 6); w < (to - from) * p.H; w += stride) {
+    const int64_t i = w / p.H, j = from + i;
+    const int h = static_cast<int>(w - i * p.H);
+    const int64_t left = j < 0 ? 0 : n - j * p.bk;
     const int cnt = left >= p.bk ? p.bk : left > 0 ? static_cast<int>(left) : 0;
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     const uint16_t *base = p.k + (begin + j * p.bk) * p.tok + h * p.head + col;
@@ -398,11 +399,15 @@ __device__ inline void choose(const uint32_t (&key)[R], int n, int topk, int32_t
   for (int e = want + wave * 64 + lane; e < topk; e += 64 * W) out[e] = -1;
 }
 
-// The lists' rows behind sequence b's `have` tiles, for KV head h
-__device__ inline void clear_rows(const SelectParams &p, int b, int h, int64_t from, int thread, int threads) {
+// The lists' rows behind sequence b's `have` tiles, of which `first` is the first
+// row, and those before the first sequence's, for KV head h
+__device__ inline void clear_rows(const SelectParams &p, int b, int h, int64_t first, int have, int thread, int threads) {
   const int64_t end = b + 1 < p.B ? seq_span(p.cu_q, b + 1, p.total_q).begin / p.bq + b + 1 : p.tile_rows;
-  for (int64_t r = from; r < end; ++r)
+  const int64_t before = b == 0 ? first : 0;
+  for (int64_t i = 0; i < before + end - first - have; ++i) {
+    const int64_t r = i < before ? i : first + have + (i - before);
     for (int e = thread; e < p.topk; e += threads) p.lists[(r * p.Hkv + h) * p.topk + e] = -1;
+  }
 }
 
 // A row (tile, KV head) of the lists from block_scores_kernel's keys: one per
@@ -419,7 +424,7 @@ __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_choose_kernel(Sele
   const int64_t first_row = q.begin / p.bq + b;
   const int have = min((q.n + p.bq - 1) / p.bq, p.tiles);
   if (tile == 0)
-    clear_rows(p, b, h, first_row + have, W > 1 ? static_cast<int>(threadIdx.x) : lane, W > 1 ? 64 * W : 64);
+    clear_rows(p, b, h, first_row, have, W > 1 ? static_cast<int>(threadIdx.x) : lane, W > 1 ? 64 * W : 64);
   if (tile >= have || nth >= p.tile_n) return;
   const int n = chosen_from(p, tk);
   const int64_t row = (static_cast<int64_t>(b) * p.tile_n + nth) * p.Hkv + h;
@@ -462,7 +467,7 @@ __global__ void __launch_bounds__(W > 1 ? 64 * W : 256) block_select_kernel(Sele
   const int64_t first_row = q.begin / p.bq + b;
   const int have = min((q.n + p.bq - 1) / p.bq, p.tiles);
   if (tile == 0)
-    clear_rows(p, b, h, first_row + have, W > 1 ? static_cast<int>(threadIdx.x) : lane, W > 1 ? 64 * W : 64);
+    clear_rows(p, b, h, first_row, have, W > 1 ? static_cast<int>(threadIdx.x) : lane, W > 1 ? 64 * W : 64);
   if (tile >= have) return;
   const int n = chosen_from(p, tk);
   const int i16 = lane & 15, g = lane >> 4;

@@ -915,6 +915,7 @@ static Tensor block_means(Tensor k, Tensor cu_seqlens_k, int64_t block_k, int64_
   const std::vector<int64_t> shape = means_shape(k, cu_seqlens_k, block_k, who);
   check_means_args(k, cu_seqlens_k, who);
   c10::DeviceGuard guard(k.device());
+  if (cu_seqlens_k.numel() == 1) return at::zeros(shape, k.options().dtype(at::kFloat));
   Tensor means = at::empty(shape, k.options().dtype(at::kFloat));
   run_block_means(means, k, cu_seqlens_k, block_k, 0, max_seqlen_k, seqlens_k, who);
   return means;
@@ -998,6 +999,7 @@ static Tensor block_select(Tensor q, Tensor means, Tensor cu_seqlens_q, Tensor c
   a.causal = !causal ? PKV_NOT_CAUSAL : rank_own ? PKV_CAUSAL_RANKED : PKV_CAUSAL;
   a.dtype = dtype_code(q, false, who);
   c10::DeviceGuard guard(q.device());
+  if (B == 0) return at::full(shape, -1, q.options().dtype(at::kInt));
   Tensor lists = at::empty(shape, q.options().dtype(at::kInt));
   a.lists = lists.data_ptr<int32_t>();
   const int64_t need = pkv_block_select_workspace_size(&a);

@@ -789,3 +789,49 @@ def test_own_blocks_ranked():
             got = bs.block_select(q, means, cu([n]), cu([n]), n, n, topk, block_q=1, sink_blocks=sink, causal=True)
             want = _select_ref(q, means, [n], [n], hkv, False, topk, 1, 64, sink, 1, True)
             assert np.array_equal(got.cpu().numpy(), want)
+
+
+def _poison(*shape, dtype):
+    """Memory that the next tensor of this size is likely to get holds no zeros."""
+    torch.cuda.synchronize()
+    x = torch.full(shape, 7, dtype=dtype, device=DEV)
+    torch.cuda.synchronize()
+    del x
+
+
+def test_rows_before_the_first_sequence():
+    """Sequences that begin behind a buffer's first rows: what lies there is no
+    block's and no tile's."""
+    k, cq, ck = rnd(700, 2, 64), torch.tensor([40, 70], dtype=torch.int32, device=DEV), \
+        torch.tensor([330, 700], dtype=torch.int32, device=DEV)
+    _poison(700 // 64 + 1, 2, 64, dtype=torch.float32)
+    means = bs.block_means(k, ck, 64)
+    assert not means[:330 // 64].any()
+    _check_means(means[330 // 64:330 // 64 + 6], k[330:].clone(), [370], 64)
+    q = rnd(80, 2, 64)
+    for bq in (1, 8):
+        _poison(80 // bq + 1, 2, 3, dtype=torch.int32)
+        lists = bs.block_select(q, means, cq, ck, 30, 370, 3, block_q=bq)
+        tiles = -(-30 // bq)
+        first = 40 // bq
+        assert (lists[:first] == -1).all() and (lists[first:first + tiles] >= 0).all()
+        assert (lists[first + tiles:] == -1).all()
+    # many blocks: scores through the workspace
+    k, ck = rnd(20000, 64), torch.tensor([330, 20000], dtype=torch.int32, device=DEV)
+    _poison(20000 // 64 + 1, 64, dtype=torch.float32)
+    means = bs.block_means(k, ck, 64)
+    assert not means[:330 // 64].any()
+    _poison(80 // 8 + 1, 1, 3, dtype=torch.int32)
+    lists = bs.block_select(q, means, cq, ck, 30, 19670, 3, block_q=8)
+    assert (lists[:5] == -1).all() and (lists[5:9] >= 0).all() and (lists[9:] == -1).all()
+
+
+def test_no_sequences():
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    q, k = rnd(40, 2, 64), rnd(300, 2, 64)
+    _poison(300 // 64, 2, 64, dtype=torch.float32)
+    means = bs.block_means(k, none, 64)
+    assert means.shape == (4, 2, 64) and not means.any()
+    _poison(40 // 8, 2, 3, dtype=torch.int32)
+    lists = bs.block_select(q, means, none, none, 0, 0, 3, block_q=8)
+    assert lists.shape == (5, 2, 3) and (lists == -1).all()
