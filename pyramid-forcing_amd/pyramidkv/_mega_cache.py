@@ -226,10 +226,10 @@ class MegaCache:
         if cu_q is None or cu_q.device != q.device:
             cu_q = ctx.cu_q[L_q] = torch.arange(0, L_q + 1, FSEQ, dtype=torch.int32, device=q.device)
         qb = q[0] if q.dtype == torch.bfloat16 else q[0].to(torch.bfloat16)
-        max_keys = self._max_keys(int(current_start // FSEQ) + C)
         if sparse is not None:
             return self._attend_sparse(qb, cu_q, C, current_start, freqs, softmax_scale, causal,
                                        sparse).view(1, L_q, H, D).to(q.dtype)
+        max_keys = self._max_keys(int(current_start // FSEQ) + C)
         if C <= int(ctx.mgr.max_attend_chunks()):
             scale = float(softmax_scale) if softmax_scale is not None else D ** -0.5
             out = ctx.mgr.attend_layer(*self._attend_args(current_start, C, freqs), qb, cu_q, scale, bool(causal),
@@ -249,8 +249,12 @@ class MegaCache:
             cu_k = self.attend_kv(current_start, C, freqs)
         else:
             cu_k = self.pack(self.plan(current_start, C), freqs)
-        # the most keys that a (chunk, head) can pack, and the workspace rows that so many chunks can fill
+        # the most keys that a (chunk, head) can pack: the workspace's room for one, less where the layer's policy
+        # keeps less (not by the frames that have come, as _max_keys has it: keys past this bound are not chosen from,
+        # and a cache may hold later frames than current_start); then the workspace rows that so many chunks can fill
         max_keys = int(mgr.max_pack_tokens()) // (int(mgr.max_attend_chunks()) * H)
+        if self.ctx.layer_max_keys:
+            max_keys = min(max_keys, self.ctx.layer_max_keys[self.layer_idx])
         n = min(int(mgr.max_pack_tokens()), C * H * max_keys)
         return sparse_ragged_attention(q, mgr.k_flat_out().view(-1, D)[:n], mgr.v_flat_out().view(-1, D)[:n], cu_q, cu_k,
                                        self.ctx.frame_seqlen, max_keys, sparse, softmax_scale=softmax_scale)

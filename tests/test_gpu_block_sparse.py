@@ -835,3 +835,52 @@ def test_no_sequences():
     _poison(40 // 8, 2, 3, dtype=torch.int32)
     lists = bs.block_select(q, means, none, none, 0, 0, 3, block_q=8)
     assert lists.shape == (5, 2, 3) and (lists == -1).all()
+
+
+def test_cache_attends_to_its_blocks_whatever_the_start():
+    """MegaCache.attend(sparse=...) bounds a head's keys by its policy, which
+    holds for queries of earlier frames than the cache has seen too."""
+    from pyramidkv import _mega_cache, factory
+    from pyramidkv._mega_cache import build_mega_caches
+    from pyramidkv.rope import wan_freqs
+    H, D, FS, W, F = 3, 128, 160, 16, 3
+    cache = build_mega_caches(1, H, D, FS, 3, 24, 4, factory.shipped_compositions(1, H, labels=[[-1, 1, 2]]),
+                              max_attend_chunks=F, device=DEV, freqs=wan_freqs(D), spatial_width=W,
+                              spatial_height=FS // W, **factory.PYRAMID_FORCING_REMAP)[0]
+    mgr, seen = cache.ctx.mgr, []
+    plain = _mega_cache.sparse_ragged_attention
+
+    def spy(q, k, v, cu_q, cu_k, max_q, max_k, *args, **kw):
+        seen.append((max_k, k.shape[0], int((cu_k[1:] - cu_k[:-1]).max()), int(cu_k[-1])))
+        return plain(q, k, v, cu_q, cu_k, max_q, max_k, *args, **kw)
+
+    _mega_cache.sparse_ragged_attention = spy
+    try:
+        for blk in range(12):
+            for mode in ("noisy", "clean"):
+                cache.update(rnd(1, F * FS, H, D), rnd(1, F * FS, H, D), blk * F * FS, cache_update_mode=mode)
+            q = rnd(1, F * FS, H, D)
+            for start in {0, blk * F * FS}:
+                dense = cache.attend(q, start)
+                ck = cache.attend_kv(start, F).clone()
+                lens = (ck[1:] - ck[:-1]).tolist()
+                k, v = (x.view(-1, D)[:sum(lens)].clone() for x in (mgr.k_flat_out(), mgr.v_flat_out()))
+                got = cache.attend(q, start, sparse=bs.BlockSparse(topk=128, block_q=80))
+                full = _lists([FS] * F, lens, H, True, 80, 64, 128, np.random.default_rng(0))
+                _attend_check(got[0], None, q[0], k, v, full, [FS] * F, lens, H, True, 80, 64)
+                _attend_check(dense[0], None, q[0], k, v, full, [FS] * F, lens, H, True, 80, 64)
+    finally:
+        _mega_cache.sparse_ragged_attention = plain
+    capacity = int(mgr.max_pack_tokens()) // (F * H)
+    kept = cache.ctx.layer_max_keys[0]
+    assert 0 < kept < capacity
+    for max_k, rows, longest, total in seen:
+        assert longest <= max_k == kept and total <= rows == F * H * kept
+    # a context without a policy's bound: the capacity
+    cache.ctx.layer_max_keys, seen[:] = [], []
+    _mega_cache.sparse_ragged_attention = spy
+    try:
+        cache.attend(q, 0, sparse=bs.BlockSparse(topk=8, block_q=80))
+    finally:
+        _mega_cache.sparse_ragged_attention = plain
+    assert seen[0][0] == capacity
