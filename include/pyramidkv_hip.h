@@ -429,7 +429,8 @@ int pkv_rotary(const pkv_rotary_args *args, pkv_stream_t stream);
  * topk] int32.  block_k: a multiple of 64 up to 1,024; block_q: 1 or more, with at
  * most 256 rows (block_q * group) a tile; topk 1 to 1,024; head_dim 64 or 128;
  * dtype bf16 or fp16.  causal (block_q 1 only): query i of a sequence of n sees
- * its keys up to keys - n + i. */
+ * its keys up to keys - n + i.  q, k, v, means and the workspaces begin at 16
+ * bytes, o at 8; strides keep their rows so. */
 
 /* causal of pkv_block_select_args.  The block that holds a token's last key may
  * hold later keys, which its mean then covers: PKV_CAUSAL takes that block

@@ -1396,6 +1396,9 @@ constexpr int64_t kMaxThreads = 0xffffffffll;
 // whole tiles and blocks (32 * 128 rows, 1,024 keys) in 32 bits
 constexpr int64_t kMaxTokens = 0x7fffffff - 4096;
 
+// what the kernels read and write in pieces of `bytes`
+static bool aligned(const void *p, uintptr_t bytes = 16) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
 static bool is_16bit(int dtype) { return dtype == PKV_DTYPE_BF16 || dtype == PKV_DTYPE_FP16; }
 
 static int check_block(int head_dim, int block_k, int dtype, const char *who) {
@@ -1432,6 +1435,7 @@ extern "C" int pkv_block_means(const pkv_block_means_args *a, pkv_stream_t strea
     return fail(PKV_ERR_INVALID, "block_means: NULL argument");
   if ((a->kv_tok_stride | a->kv_head_stride) & 7)
     return fail(PKV_ERR_INVALID, "block_means: strides must keep 16-byte rows aligned");
+  if (!aligned(a->k) || !aligned(a->means)) return fail(PKV_ERR_INVALID, "block_means: k and means must begin at 16 bytes");
   if (a->num_seqs > kMaxThreads / 256) return fail(PKV_ERR_UNSUPPORTED, "block_means: too many sequences");
   MeansParams p{};
   p.k = a->k; p.means = a->means; p.cu = a->cu_seqlens_k; p.used = a->seqlens_k;
@@ -1590,6 +1594,8 @@ extern "C" int pkv_block_select(const pkv_block_select_args *a, void *workspace,
     return fail(PKV_ERR_INVALID, "block_select: NULL argument");
   if ((a->q_tok_stride | a->q_head_stride) & 7)
     return fail(PKV_ERR_INVALID, "block_select: strides must keep 16-byte rows aligned");
+  if (!aligned(a->q) || !aligned(a->means) || !aligned(workspace))
+    return fail(PKV_ERR_INVALID, "block_select: q, means and the workspace must begin at 16 bytes");
   const SelectPlan s = select_plan(a);
   if (s.bytes > 0 && (!workspace || workspace_bytes < s.bytes))
     return fail(PKV_ERR_CAPACITY, "block_select: workspace of %lld bytes, %lld needed",
@@ -1737,6 +1743,8 @@ extern "C" int pkv_block_attn(const pkv_block_attn_args *a, void *workspace, int
   if (((a->q_tok_stride | a->q_head_stride | a->kv_tok_stride | a->kv_head_stride) & 7) ||
       ((a->o_tok_stride | a->o_head_stride) & 3))
     return fail(PKV_ERR_INVALID, "block_attn: strides must keep 16-byte rows aligned");
+  if (!aligned(a->q) || !aligned(a->k) || !aligned(a->v) || !aligned(a->o, 8) || !aligned(workspace))
+    return fail(PKV_ERR_INVALID, "block_attn: q, k, v and the workspace must begin at 16 bytes, o at 8");
   // buffer offsets within one step of keys are 32-bit; a step's bound is its keys
   // times the stride, which must hold a whole row
   if (a->kv_tok_stride < a->head_dim || a->kv_tok_stride * 2 * kSub > 0x7fffffff)

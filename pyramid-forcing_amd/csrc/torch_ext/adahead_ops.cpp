@@ -929,6 +929,7 @@ static void block_means_(Tensor means, Tensor k, Tensor cu_seqlens_k, int64_t bl
   TORCH_CHECK(means.device() == k.device() && means.scalar_type() == at::kFloat && means.is_contiguous() &&
                   means.sizes() == at::IntArrayRef(shape),
               who, ": means must be contiguous float32 ", at::IntArrayRef(shape), " on ", k.device());
+  check_aligned(means, who, "means");
   TORCH_CHECK(last >= 1, who, ": last must be at least 1");
   c10::DeviceGuard guard(k.device());
   run_block_means(means, k, cu_seqlens_k, block_k, last, max_seqlen_k, seqlens_k, who);

@@ -240,3 +240,16 @@ def test_meta_refusals(block):
                  lambda: ops.block_select(q, means, none, none, 5, 50, 3, 4, 64)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_refusals_of_unaligned_pointers():
+    """Read and written in 16-byte pieces (o in 8-byte ones)."""
+    lib = A.lib()
+    for name in ("k", "means"):
+        _refused(lib.pkv_block_means(ctypes.byref(_means(**{name: FAKE + 8})), None))
+    for name in ("q", "means"):
+        _refused(lib.pkv_block_select(ctypes.byref(_select(**{name: FAKE + 8})), FAKE, 1 << 40, None))
+    _refused(lib.pkv_block_select(ctypes.byref(_select(max_seqlen_k=64 * 20000)), FAKE + 8, 1 << 40, None))
+    for name, off in (("q", 8), ("k", 8), ("v", 2), ("o", 4)):
+        _refused(lib.pkv_block_attn(ctypes.byref(_attn(**{name: FAKE + off})), FAKE, 1 << 40, None))
+    _refused(lib.pkv_block_attn(ctypes.byref(_attn(block_q=1, max_seqlen_q=1, topk=64)), FAKE + 8, 1 << 40, None))

@@ -884,3 +884,11 @@ def test_cache_attends_to_its_blocks_whatever_the_start():
     finally:
         _mega_cache.sparse_ragged_attention = plain
     assert seen[0][0] == capacity
+
+
+def test_means_off_16_bytes_are_refused():
+    k, c = rnd(200, 64), cu([200])
+    buf = torch.zeros(200 // 64 + 1 + 1, 64, device=DEV).view(-1)
+    with pytest.raises(RuntimeError):
+        bs.block_means(k, c, 64, out=buf[1:1 + 4 * 64].view(4, 64), last=1)
+    bs.block_means(k, c, 64, out=buf[4:4 + 4 * 64].view(4, 64), last=1)
