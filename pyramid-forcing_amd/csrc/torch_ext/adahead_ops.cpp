@@ -13,6 +13,9 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/custom_class.h>
 #include <torch/library.h>
 
@@ -1754,6 +1757,34 @@ TORCH_LIBRARY_IMPL(adahead, CUDA, m) {
 
 // Ops whose only tensor arguments may live on the host, or that take none,
 // dispatch the same implementation whatever the tensor backend.
+// No derivative formulas here: a gradient or a tangent that is asked for raises
+// (rope.rotary has its own, and calls the op below them).  torch's own fallback
+// does so too, at up to 0.5 us more of the host's time a call.
+static void no_derivative(const c10::OperatorHandle &op, c10::DispatchKeySet keys, torch::jit::Stack *stack) {
+  std::vector<at::Tensor> wanted;
+  const bool grad = at::GradMode::is_enabled();
+  for (const c10::IValue &v : torch::jit::last(*stack, op.schema().arguments().size())) {
+    if (!v.isTensor()) continue;
+    const at::Tensor &t = v.toTensor();
+    if (!t.defined() || !torch::autograd::impl::get_autograd_meta(t)) continue;  // (has neither)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), op.schema().name(), ": forward derivatives are not implemented");
+    if (grad && t.requires_grad()) wanted.push_back(t);
+  }
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+  if (wanted.empty()) return;
+  auto node = std::make_shared<torch::autograd::NotImplemented>(op.schema().name());
+  node->set_next_edges(torch::autograd::collect_next_edges(wanted));
+  for (const c10::IValue &v : torch::jit::last(*stack, op.schema().returns().size()))
+    for (const at::Tensor &t : v.isTensor() ? std::vector<at::Tensor>{v.toTensor()} : v.toTensorVector())
+      if (at::isFloatingType(t.scalar_type())) torch::autograd::set_history(t, node);
+}
+
+TORCH_LIBRARY_IMPL(adahead, Autograd, m) {
+  for (const char *name : {"rotary", "block_means", "block_select", "block_sparse_attention"})
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
+  m.impl("block_means_", torch::autograd::autogradNotImplementedFallback());
+}
+
 TORCH_LIBRARY_IMPL(adahead, CompositeExplicitAutograd, m) {
   m.impl("mega_state_perhead_size", adahead::mega_state_perhead_size);
   m.impl("mega_evict_merge_workspace_size", adahead::mega_evict_merge_workspace_size);

@@ -27,7 +27,7 @@ to find one.
 
 All run on the current stream without a host synchronisation, in workspaces of
 torch's allocator, and may be captured into a graph.  They have no backward
-pass.  Rows of the attention's results that no sequence owns, and those past
+pass: a gradient or a tangent through them raises.  Rows of the attention's results that no sequence owns, and those past
 max_seqlen_q in theirs, are not written.
 """
 from __future__ import annotations

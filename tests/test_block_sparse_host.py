@@ -253,3 +253,25 @@ def test_refusals_of_unaligned_pointers():
     for name, off in (("q", 8), ("k", 8), ("v", 2), ("o", 4)):
         _refused(lib.pkv_block_attn(ctypes.byref(_attn(**{name: FAKE + off})), FAKE, 1 << 40, None))
     _refused(lib.pkv_block_attn(ctypes.byref(_attn(block_q=1, max_seqlen_q=1, topk=64)), FAKE + 8, 1 << 40, None))
+
+
+def test_derivatives_that_are_not_there_raise():
+    """Not a warning and no gradient."""
+    from torch.autograd import forward_ad as fw
+    m = dict(device="meta")
+    ops = _ops.ops()
+    q, k = torch.empty(10, 8, 128, dtype=torch.bfloat16, **m), torch.empty(100, 2, 128, dtype=torch.bfloat16, **m)
+    cu, lists = torch.empty(3, dtype=torch.int32, **m), torch.empty(4, 2, 3, dtype=torch.int32, **m)
+    pos, f = torch.empty(10, dtype=torch.int64, **m), torch.empty(32, dtype=torch.float64, **m)
+    calls = dict(means=(lambda x, y: ops.block_means(y, cu, 64), k),
+                 attend=(lambda x, y: ops.block_sparse_attention(x, y, y, cu, cu, 5, lists, 0.1, 4, 64)[0], q),
+                 rotary=(lambda x, y: ops.rotary(x, None, pos, f, [32], True, 1.0, False)[0], q))
+    for name, (call, x) in calls.items():
+        pair = lambda z: (z, k) if x is q else (q, z)
+        out = call(*pair(x.clone().requires_grad_()))
+        with pytest.raises(RuntimeError, match="not implemented"):
+            out.sum().backward()
+        with fw.dual_level(), pytest.raises(NotImplementedError):
+            call(*pair(fw.make_dual(x, torch.empty_like(x))))
+    # what chooses blocks is no function to derive, and its result no floating number
+    assert not ops.block_select(q.clone().requires_grad_(), torch.empty(3, 2, 128, **m), cu, cu, 5, 50, 3, 4, 64).requires_grad
