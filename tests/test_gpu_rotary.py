@@ -333,3 +333,22 @@ def test_rotary_refuses_frequencies_that_want_gradients():
             rope.rotary(x, pos, f)
     with torch.no_grad():
         assert torch.equal(rope.rotary(q, pos, f), q)
+
+
+@pytest.mark.parametrize("far", [1, 100, 1 << 20])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_rotary_rounds_sine_and_cosine_once(interleaved, far):
+    """fp32, scale 1, u = 2^-24: c and s are off by u of themselves, one of the
+    two products by u (the other goes into the sum as it is, or by u too), the sum
+    by u of the result: 2 u (|a c| + |b s|) + u |y|.  The angle in 64 bits is off
+    by 2^-51 of itself on either side.  Second-order terms: a factor 1 + 2^-20."""
+    f, pos = rope.rotary_frequencies(128, device=DEV)[0], torch.randint(-far, far + 1, (3000,), device=DEV)
+    x = torch.randn(3000, 2, 128, device=DEV)
+    got = rope.rotary(x, pos, f, interleaved=interleaved).double()
+    iu, iw = (slice(0, 128, 2), slice(1, 128, 2)) if interleaved else (slice(0, 64), slice(64, 128))
+    a = (pos.double()[:, None] * f)[:, None]
+    c, s, u, w = a.cos(), a.sin(), x[..., iu].double(), x[..., iw].double()
+    off = 2.0 ** -50 * a.abs() * (u.abs() + w.abs())
+    for at, y, size in ((iu, u * c - w * s, (u * c).abs() + (w * s).abs()), (iw, u * s + w * c, (u * s).abs() + (w * c).abs())):
+        bound = 2.0 ** -24 * (2 * size + y.abs()) * (1 + 2.0 ** -20) + off
+        assert ((got[..., at] - y).abs() <= bound).all()
