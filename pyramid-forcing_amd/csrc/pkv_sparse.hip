@@ -1476,15 +1476,22 @@ struct SelectPlan {
 };
 
 // Scores and choice in one launch where that reads few means more than once,
-// measured against three launches, microseconds each (head_dim 128):
-// * up to 128 blocks (a wave a row), up to kFusedBytes of means in all: 1,024
-//   rows of 64 blocks 7.6 against 11.3, 4,094 of 64 12.0 against 13.0, but
-//   32,768 of 64 97 against 33;
+// measured against three launches (two without the sums'), microseconds each:
+// * up to 128 blocks (a wave a row) where no other tile of the sequence reads the
+//   same means and the sum is short: 32 single tokens of 64 blocks and head_dim 128
+//   7.2 against 10.4, 4,096 26.5 against 46.6, of 128 blocks 47.8 against 70.6;
+// * up to kFusedRow columns of means a row and kFusedBytes in all (causal rows
+//   counted by the blocks that they see on average): 2,048 rows of 32 blocks and
+//   head_dim 128 (32 MB) 8.4 against 10.7, 4,000 causal ones of 32 to 63 and head_dim
+//   64 (46 MB) 10.5 against 11.4, 2,048 of 64 and 128 (64 MB) 11.0 alike, 4,094 of
+//   32 and 128 (64 MB) 14.6 against 12.1, 4,094 of 64 (128 MB) 20.3 against 12.4,
+//   16,384 71 against 29; and 156 rows of 128 blocks and head_dim 128 (10 MB) 15.6
+//   against 13.1, of 64 blocks 11.2 against 13.2;
 // * more, where no other tile of the sequence reads the same means (single
 //   tokens) and the rows fill the chip: 128 rows of 512 blocks 14.4 against
 //   18.1, 512 of 2,048 106 against 124, but 8 of 2,048 37 against 19, and
 //   468 rows of 13 tiles a sequence and 320 blocks 21.7 against 16.8.
-constexpr int64_t kFusedBytes = 140ll << 20;
+constexpr int64_t kFusedBytes = 48ll << 20, kFusedRow = 64 * 128;
 constexpr int64_t kFusedMost = 4096, kFusedRows = 64;
 
 static int check_select(const pkv_block_select_args *a) {
@@ -1516,10 +1523,15 @@ static SelectPlan select_plan(const pkv_block_select_args *a) {
   if (s.tiles == 0) s.tiles = 1;  // (the lists' rows are written all the same)
   const int64_t heads = static_cast<int64_t>(a->num_batches) * a->num_heads_kv;
   const int64_t rows = heads * s.tiles;
-  s.fused = s.nb <= 128 ? rows * s.nb * a->head_dim * 4 <= kFusedBytes
-                        : s.tiles == 1 && rows >= kFusedRows && s.nb <= kFusedMost;
-  if (s.fused) return s;
   const bool sums = a->block_q * (a->num_heads_q / a->num_heads_kv) > kSumRowsInline;
+  int64_t keys = a->max_seqlen_k;  // that a row sees on average
+  if (a->causal) keys -= (a->max_seqlen_q < keys ? a->max_seqlen_q : keys) / 2;
+  const int64_t means = rows * (keys / a->block_k + 1) * a->head_dim * 4;
+  if (s.nb <= 128)
+    s.fused = (s.tiles == 1 && !sums) || (s.nb * a->head_dim <= kFusedRow && means <= kFusedBytes);
+  else
+    s.fused = s.tiles == 1 && rows >= kFusedRows && s.nb <= kFusedMost;
+  if (s.fused) return s;
   const int64_t per_tile = heads * (s.nb * 4 + (sums ? a->head_dim * 8 : 0));
   s.tile_n = kSelectWorkspace / (per_tile > 0 ? per_tile : 1) / 16 * 16;
   if (s.tile_n < 16) s.tile_n = 16;

@@ -275,3 +275,19 @@ def test_derivatives_that_are_not_there_raise():
             call(*pair(fw.make_dual(x, torch.empty_like(x))))
     # what chooses blocks is no function to derive, and its result no floating number
     assert not ops.block_select(q.clone().requires_grad_(), torch.empty(3, 2, 128, **m), cu, cu, 5, 50, 3, 4, 64).requires_grad
+
+
+def test_selection_in_one_launch_where_few_means_are_read_again():
+    """One launch needs no workspace.  Rows that share their sequence's means: up
+    to 48 MiB of them in all; single tokens, which share none: any number."""
+    need = lambda **kw: A.lib().pkv_block_select_workspace_size(ctypes.byref(_select(**dict(
+        dict(block_q=1, num_heads_q=8, num_heads_kv=2, total_q=1 << 20, total_k=1 << 22), **kw))))
+    assert need(max_seqlen_q=700, max_seqlen_k=4000) == 0       # 1,400 rows of 63 blocks of 512 bytes: 43 MiB
+    assert need(max_seqlen_q=2047, max_seqlen_k=4000) > 0       # 123 MiB
+    assert need(max_seqlen_q=1200, max_seqlen_k=2047) == 0      # 37 MiB
+    assert need(max_seqlen_q=2047, max_seqlen_k=2047) > 0       # 62 MiB
+    assert need(max_seqlen_q=2047, max_seqlen_k=2047, causal=1) == 0  # half of that on average
+    assert need(max_seqlen_q=4000, max_seqlen_k=4000, causal=1) > 0
+    assert need(max_seqlen_q=4000, max_seqlen_k=1000, causal=1) == 0  # most rows see nothing
+    assert need(max_seqlen_q=1, max_seqlen_k=8000, num_batches=4096) == 0
+    assert need(max_seqlen_q=13, max_seqlen_k=8000) > 0         # 125 blocks of 128 columns: too long for a wave

@@ -892,3 +892,22 @@ def test_means_off_16_bytes_are_refused():
     with pytest.raises(RuntimeError):
         bs.block_means(k, c, 64, out=buf[1:1 + 4 * 64].view(4, 64), last=1)
     bs.block_means(k, c, 64, out=buf[4:4 + 4 * 64].view(4, 64), last=1)
+
+
+@pytest.mark.parametrize("n,blocks,hkv,causal", [(2100, 64, 2, False), (4096, 64, 2, True), (600, 100, 1, False), (1300, 20, 2, True)])
+def test_select_of_many_rows(n, blocks, hkv, causal):
+    """Prompts of few blocks, in one launch or in several."""
+    q, means = rnd(n, 2 * hkv, 128), torch.randn(blocks + 1, hkv, 128, device=DEV)
+    keys = blocks * 64 - 17
+    got = _run_select(q, means, [n], [keys], hkv, False, 7, 1, 64, 1, 2, causal)
+    tile = q.view(n, hkv, 2, 128).double().sum(dim=2).cpu()
+    score = torch.matmul(tile.transpose(0, 1), means[:blocks].cpu().double().permute(1, 2, 0).contiguous()).float()
+    limit = (keys - n + 1 + torch.arange(n)).clamp(min=0) if causal else torch.full((n,), keys)
+    here = -(-limit // 64)                                              # blocks of a token
+    j = torch.arange(blocks)
+    score = torch.where((j < 1) | (j >= here[:, None] - 2), INF, score)
+    score = torch.where(j < here[:, None], score, -INF)
+    want = score.sort(dim=-1, descending=True, stable=True).indices[..., :7]
+    want = torch.where(want < here[:, None], want, 1 << 20).sort(dim=-1).values
+    want = torch.where(want < 1 << 20, want, -1).transpose(0, 1)
+    assert torch.equal(got[:n].cpu().long(), want) and (got[n:] == -1).all()
