@@ -13,7 +13,6 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/custom_class.h>
@@ -1759,7 +1758,9 @@ TORCH_LIBRARY_IMPL(adahead, CUDA, m) {
 // dispatch the same implementation whatever the tensor backend.
 // No derivative formulas here: a gradient or a tangent that is asked for raises
 // (rope.rotary has its own, and calls the op below them).  torch's own fallback
-// does so too, at up to 0.5 us more of the host's time a call.
+// does so too, at up to 0.5 us more of the host's time a call.  Not for
+// block_select, whose result is no floating number, nor block_means_, which
+// writes a cache's means without any history.
 static void no_derivative(const c10::OperatorHandle &op, c10::DispatchKeySet keys, torch::jit::Stack *stack) {
   std::vector<at::Tensor> wanted;
   const bool grad = at::GradMode::is_enabled();
@@ -1780,9 +1781,8 @@ static void no_derivative(const c10::OperatorHandle &op, c10::DispatchKeySet key
 }
 
 TORCH_LIBRARY_IMPL(adahead, Autograd, m) {
-  for (const char *name : {"rotary", "block_means", "block_select", "block_sparse_attention"})
+  for (const char *name : {"rotary", "block_means", "block_sparse_attention"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
-  m.impl("block_means_", torch::autograd::autogradNotImplementedFallback());
 }
 
 TORCH_LIBRARY_IMPL(adahead, CompositeExplicitAutograd, m) {

@@ -26,9 +26,10 @@ rows of [kv_heads, topk] int32): no prefix sum over ragged lengths is needed
 to find one.
 
 All run on the current stream without a host synchronisation, in workspaces of
-torch's allocator, and may be captured into a graph.  They have no backward
-pass: a gradient or a tangent through them raises.  Rows of the attention's results that no sequence owns, and those past
-max_seqlen_q in theirs, are not written.
+torch's allocator, and may be captured into a graph.  They have no derivatives:
+a gradient or a tangent through means or attention raises; the choice of blocks,
+and means written in place (out=), carry none.  Rows of the attention's results
+that no sequence owns, and those past max_seqlen_q in theirs, are not written.
 """
 from __future__ import annotations
 

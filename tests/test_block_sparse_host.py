@@ -291,3 +291,19 @@ def test_selection_in_one_launch_where_few_means_are_read_again():
     assert need(max_seqlen_q=4000, max_seqlen_k=1000, causal=1) == 0  # most rows see nothing
     assert need(max_seqlen_q=1, max_seqlen_k=8000, num_batches=4096) == 0
     assert need(max_seqlen_q=13, max_seqlen_k=8000) > 0         # 125 blocks of 128 columns: too long for a wave
+
+
+def test_choices_and_means_in_place_carry_no_derivative():
+    """A cache's means keep no history of the keys that they were brought up to
+    date from, and blocks are chosen for queries with a tangent too."""
+    from torch.autograd import forward_ad as fw
+    m = dict(device="meta")
+    ops = _ops.ops()
+    q, k = torch.empty(10, 8, 128, dtype=torch.bfloat16, **m), torch.empty(100, 2, 128, dtype=torch.bfloat16, **m)
+    cu, means = torch.empty(3, dtype=torch.int32, **m), torch.empty(3, 2, 128, **m)
+    for _ in range(2):
+        ops.block_means_(means, k.clone().requires_grad_(), cu, 64, 1)
+        assert not means.requires_grad and means.grad_fn is None
+    with fw.dual_level():
+        lists = ops.block_select(fw.make_dual(q, torch.empty_like(q)), means, cu, cu, 5, 50, 3, 4, 64)
+    assert lists.dtype == torch.int32 and not lists.requires_grad
