@@ -16,7 +16,7 @@
 // Bound by memory: every element is read and written once.  A workgroup takes
 // a few tokens, computes each (token, pair)'s sine and cosine once in LDS and
 // applies them to all heads of q and k in 16-byte accesses.  4,680 rows of 12
-// heads of 128 (bf16, 29 MB read and written) in 7.1 us, 4.1 TB/s; 8,191 rows of 20
+// heads of 128 (bf16, 29 MB read and written) in 7.3 us, 4.0 TB/s; 8,191 rows of 20
 // heads of 80 (fp32, 105 MB) in 18 us under the profiler and 25 a call, 4.2 TB/s (a
 // copy of 1 GiB moves 4.8); 16 rows of 40 heads in 3.6, the launch and the chain of
 // position, angle and store.  Reading q ahead of the angles was no faster.

@@ -957,8 +957,8 @@ struct TileCopies {
 // adds up.
 //
 // 468 tiles of 120 rows over 6,400 keys each (bf16, head_dim 128; 184 GFLOP) take
-// 220 to 237 us, 775 to 835 TFLOP/s, where a large library product reaches 1,200 on
-// the same card.  Matrix units are busy 56% of the time of the units that have
+// 220 to 237 us, 775 to 835 TFLOP/s, where a large library product of such values
+// reaches 1,200 to 1,281 on the same cards.  Matrix units are busy 56% of the time of the units that have
 // work; without the copies it takes 178 us, without LDS reads too 145, without
 // exponentials too 121: copies, fragment reads and exponentials each take time
 // that the matrix instructions of two waves a SIMD do not cover.  A copy serves one
