@@ -956,17 +956,17 @@ struct TileCopies {
 // divides the list over as many workgroups, whose parts block_attn_join_kernel
 // adds up.
 //
-// 468 tiles of 120 rows over 6,400 keys each (bf16, head_dim 128; 184 GFLOP) take
-// 220 to 237 us, 775 to 835 TFLOP/s, where a large library product of such values
-// reaches 1,200 to 1,281 on the same cards.  Matrix units are busy 56% of the time of the units that have
-// work; without the copies it takes 178 us, without LDS reads too 145, without
-// exponentials too 121: copies, fragment reads and exponentials each take time
+// 468 tiles of 120 rows over 6,400 keys each (bf16, head_dim 128; 184 GFLOP) take 220
+// to 237 us, 775 to 835 TFLOP/s, where a large library product of such values reaches
+// 1,200 to 1,281 on the same cards.  Matrix units are busy 56% of the time of the
+// units that have work; without the copies it takes 178 us, without LDS reads too 145,
+// without exponentials too 121: copies, fragment reads and exponentials each take time
 // that the matrix instructions of two waves a SIMD do not cover.  A copy serves one
-// tile; what a head's tiles list in common (here 24 sink and recent blocks of 100)
-// is copied for each of them.  Not faster:
-// steps of 32 keys in a ring of four; the scores of the next step beside the
-// exponentials of this one (219 to 240 in all orders tried); 64 rows a wave (260);
-// raised wave priority; touching the next blocks ahead (235 to 268).
+// tile; what a head's tiles list in common (here 24 sink and recent blocks of 100) is
+// copied for each of them.  Not faster: steps of 32 keys in a ring of four; the scores
+// of the next step beside the exponentials of this one (219 to 240 in all orders
+// tried); 64 rows a wave (260); raised wave priority; touching the next blocks ahead
+// (235 to 268).
 template <int D, int W, int STEP, bool F16>
 __global__ void __launch_bounds__(64 * W, 2) block_attn_tile_kernel(BlockAttnParams p) {
   constexpr int ROW = 2 * D, TILE = STEP * ROW;  // bytes
